@@ -298,6 +298,130 @@ UOCR_API int uocr_op_moe_ffn_rows(const uocr_op_moe_weights *m, const void *x, c
 UOCR_API int uocr_op_moe_ffn_rows_static(const uocr_op_moe_weights *m, const void *x, const void *norm_w,
                                          const void *residual, uint32_t rows, int norm_topk, void *out);
 
+/* ---- serving several sequences: a paged KV cache -------------------------- */
+
+/* The operators of this part serve several sequences at once (the engine
+ * serves one, on a contiguous ring cache); the reference has no counterpart.
+ * Their host arguments are checked before anything is launched.  What lives on
+ * the device (tables, lengths, positions, starts, sampling settings) is checked
+ * by the kernels, as said at each, so a bad value never leads out of range.
+ * Device pointers belong to device 0; operands that another stream writes have
+ * to be finished first.  All of them can be captured (uocr_hip_capture_begin),
+ * with no allocation inside; a replay reads the device-side values anew. */
+
+/* A paged KV cache.  Token p of sequence s stands in page
+ * page_table[s * table_stride + p / page_tokens], at slot p % page_tokens of
+ * each KV head; a table entry outside [0, n_pages) is an absent page, which
+ * holds no tokens.  A page is [kv_heads][page_tokens][head_dim] values of
+ * qtype (1 fp16, 3 Q8_0) in k and in v; Q8_0 pages have fp16 scales
+ * [kv_heads][page_tokens][head_dim / 64] in k_scales and v_scales.  From one
+ * page to the next are page_stride values (0: pages without gaps) and
+ * page_stride / 64 scales, so that the layers of a model can share a page.
+ * Limits: head_dim 64 or 128; page_tokens a power of two up to 65536;
+ * page_stride a multiple of head_dim, at least the page; k and v on 16-byte,
+ * scales on 4-byte boundaries; table_stride * page_tokens below 2^31. */
+typedef struct uocr_op_kv_pages {
+    uint32_t qtype;
+    uint32_t kv_heads, head_dim;
+    uint32_t page_tokens, n_pages;
+    uint32_t n_seqs, table_stride;
+    uint32_t reserved0; /* 0 */
+    uint64_t page_stride;
+    void *k, *v;
+    void *k_scales, *v_scales;
+    const int32_t *page_table;
+} uocr_op_kv_pages;
+
+/* Writes the keys and values of `tokens` new tokens into their pages and
+ * rotates queries and keys to their positions (split-half RoPE over the whole
+ * head, angle = position * rope_theta^(-2 i / head_dim), exact to 2^-25 turns
+ * for every int32 position; rope_theta 0: no rotation).  Token i belongs to
+ * sequence seqs[i] (NULL: sequence i) at positions[i].  Rows are
+ * [heads][head_dim] fp16 (k, v: [kv_heads][head_dim]), q_stride .. v_stride
+ * values from one token to the next (at least a row).  q NULL: no queries;
+ * q_out may be q and k_out may be k (with the same stride); k_out NULL: the
+ * rotated keys go to the pages alone.  Q8_0 pages are quantised from the fp32
+ * rotated values with the rule of uocr_quantize_rows; a group with a value
+ * that is not finite gets a NaN scale.  A token whose sequence or position is
+ * out of range (a padding row: -1) is left out: its output rows and the pages
+ * keep what they hold.  A token whose page is absent gets its q_out and k_out
+ * but is not stored.  A (sequence, position) that comes twice in a call is
+ * stored by one of its tokens, or in a mix of both.  Beside
+ * uocr_op_attention_block's KV write. */
+UOCR_API int uocr_op_kv_append(const uocr_op_kv_pages *pages, uint32_t tokens, const int32_t *seqs,
+                               const int32_t *positions, uint32_t heads, float rope_theta, const void *q,
+                               uint64_t q_stride, void *q_out, uint64_t q_out_stride, const void *k, uint64_t k_stride,
+                               void *k_out, uint64_t k_out_stride, const void *v, uint64_t v_stride);
+
+/* Reads cached tokens back as fp16 rows (Q8_0: fp16(q * scale), rounded once):
+ * k_out and v_out [tokens][kv_heads][head_dim], strides in values; either may
+ * be NULL.  Tokens out of range or in absent pages give zeros.  For a prompt
+ * that continues a cached prefix (uocr_op_packed_attention). */
+UOCR_API int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens, const int32_t *seqs,
+                               const int32_t *positions, void *k_out, uint64_t k_out_stride, void *v_out,
+                               uint64_t v_out_stride);
+
+/* Bytes of uocr_op_paged_attention's workspace (any contents), or 0 for sizes
+ * that it refuses. */
+UOCR_API size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads,
+                                                        uint32_t head_dim);
+
+/* Attention of one new token of each sequence over its first lengths[s]
+ * cached tokens (device, the new token counted; clamped to 0 and the table):
+ * out[s][h] = sum_j p_j v_j, p = softmax_j(scale q . k_j), KV head
+ * h / (heads / kv_heads).  q and out fp16 [n_seqs][heads][head_dim], strides in
+ * values from one sequence to the next (out may be q); scale 0: 1 /
+ * sqrt(head_dim).  fp32 softmax and sums; probabilities and Q8_0 values enter
+ * the products in fp16.  Tokens in absent pages are left out; where none is
+ * left the row is zero.  Beside uocr_op_attention_decode. */
+UOCR_API int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_t *lengths, uint32_t heads, float scale,
+                                     const void *q, uint64_t q_stride, void *workspace, void *out,
+                                     uint64_t out_stride);
+
+/* Causal attention of n_seqs prompts packed behind each other: prompt s has
+ * query rows q_starts[s] .. q_starts[s + 1] - 1 and key rows k_starts[s] ..
+ * k_starts[s + 1] - 1 (int32 [n_seqs + 1] on the device, not decreasing,
+ * clamped to q_tokens and k_tokens; k_starts NULL: q_starts).  Its queries are
+ * the last of its keys: query i of nq sees keys j <= i + nk - nq of nk, so
+ * rows behind a cached prefix have more keys than queries.  A row that sees
+ * no key is zero; rows outside every prompt keep what they hold.  q and out
+ * fp16 [q_tokens][heads][head_dim], k and v [k_tokens][kv_heads][head_dim],
+ * strides in values from one token to the next (below 2^22); query head h
+ * takes KV head h / (heads / kv_heads); head_dim 64 or 128; scale 0: 1 /
+ * sqrt(head_dim).  fp32 softmax and sums, fp16 probabilities.  Values that a
+ * row does not see never reach it, not finite ones either.  Beside
+ * uocr_op_prefill_attention. */
+UOCR_API int uocr_op_packed_attention(uint32_t n_seqs, const int32_t *q_starts, uint32_t q_tokens,
+                                      const int32_t *k_starts, uint32_t k_tokens, uint32_t heads, uint32_t kv_heads,
+                                      uint32_t head_dim, float scale, const void *q, uint64_t q_stride, const void *k,
+                                      uint64_t k_stride, const void *v, uint64_t v_stride, void *out,
+                                      uint64_t out_stride);
+
+/* Bytes of uocr_op_sample's workspace (any contents). */
+UOCR_API size_t uocr_op_sample_workspace_bytes(uint32_t rows, uint32_t vocab);
+
+/* A token of each row of logits ([rows][vocab], `stride` values apart; type 1
+ * fp16, 2 fp32) with the row's settings (device arrays [rows]; NULL: off) and
+ * its uniform number in [0, 1).  With w_i = exp((x_i - max x) / temperature),
+ *   top_k > 0 keeps the k largest logits, equal ones by lowest id;
+ *   top_p < 1 keeps of these, largest first, those whose predecessors' sum is
+ *     below top_p times the sum of all (the first always);
+ *   min_p keeps of these the ones with w_i >= min_p (a maximum always);
+ * and the token is the lowest id whose running sum of kept weights, by id, is
+ * over uniform times their sum.  tokens[row] is that id, probs[row] (may be
+ * NULL) its weight over the sum.  A temperature that is not above 0 takes the
+ * largest logit, the lowest id of equal ones, with probability 1.  NaN logits
+ * count as -inf, -inf ones are never taken; a row without any other gives id 0
+ * and probability 0, and with a +inf one only those have weight.  top_p that
+ * is not below 1 and min_p that is not above 0 are off; a uniform number below
+ * 0 or NaN is 0, one from 1 up the number before 1.  Weights are summed as
+ * integers (62 bits less the vocabulary's), so the order of sums never matters;
+ * vocab <= 2^24.  Beside uocr_op_lm_head_argmax; logits come from
+ * uocr_op_gemm. */
+UOCR_API int uocr_op_sample(uint32_t type, uint32_t rows, uint32_t vocab, const void *logits, uint64_t stride,
+                            const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                            const float *uniform, void *workspace, int32_t *tokens, float *probs);
+
 /* ---- 3. device plumbing ---------------------------------------------------- */
 UOCR_API int uocr_hip_device_count(void);
 /* Device memory on the library's device, zero-filled (a fresh operator

@@ -1,0 +1,653 @@
+/*
+ * uocr_kv_pages.hip - the paged KV cache on gfx950: appending tokens with the
+ * position rotation applied, reading them back as rows, and the attention of
+ * one new token of each sequence.
+ */
+#include "uocr_gemm.h"
+#include "uocr_serve.h"
+
+#include <math.h>
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+constexpr u32 APPEND_TOKENS = 8; /* most tokens of a block */
+
+/* ---- append ----------------------------------------------------------------- */
+
+/* y1 = x1 cos - x2 sin, y2 = x1 sin + x2 cos on the pairs (i, i + D/2) of a
+ * head.  A row is D/16 lanes, each 8 values of the low half and their partners.
+ * Bound by HBM: every row is read and written once.  The angle is formed in
+ * turns in fp64 and reduced to half a turn before the fp32 sine and cosine
+ * (position 10^6 in fp32 would be off by 0.06 radians); a block computes them
+ * once per token, in LDS, for all its heads. */
+template <int D, bool Q8>
+__global__ __launch_bounds__(256) void k_kv_append(uocr_append_args a, u32 tpb) {
+    constexpr u32 LPR = D / 16;
+    __shared__ float2 cs[APPEND_TOKENS][D / 2];
+    __shared__ int page_of[APPEND_TOKENS], pos_of[APPEND_TOKENS];
+    const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
+    if (a.rotate) {
+        for (u32 i = t; i < nt * (D / 2); i += 256u) {
+            const u32 tok = i / (D / 2), d = i % (D / 2);
+            const double turns = (double)a.pos[t0 + tok] * (exp2((double)d * (-2.0 / D) * a.log2_theta) * 0.15915494309189535);
+            float2 v;
+            sincospif((float)(2.0 * (turns - rint(turns))), &v.y, &v.x);
+            cs[tok][d] = v;
+        }
+    }
+    if (t < nt) {
+        const int seq = a.seqs != nullptr ? a.seqs[t0 + t] : (int)(t0 + t), pos = a.pos[t0 + t];
+        const bool in = seq >= 0 && (u32)seq < a.kv.n_seqs && pos >= 0 && ((u32)pos >> a.kv.shift) < a.kv.table_stride;
+        pos_of[t] = in ? pos : -1;
+        page_of[t] = in ? kv_page(a.kv, seq, (u32)pos) : -1;
+    }
+    __syncthreads();
+    const u32 kvh = a.kv.heads, rows = a.heads + 2u * kvh, items = nt * rows * LPR;
+    for (u32 i = t; i < items; i += 256u) {
+        const u32 lane = i % LPR, tok = i / LPR / rows, r = i / LPR % rows;
+        const int pos = pos_of[tok];
+        if (pos < 0) continue; /* a padding row: the whole row's lanes leave together */
+        const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
+        const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
+        const uint16_t *src = (is_q ? a.q + (t0 + tok) * a.qs : is_v ? a.v + (t0 + tok) * a.vs : a.k + (t0 + tok) * a.ks) + h * D + 8u * lane;
+        U4H8 lo, hi;
+        lo.u = load_any(src);
+        hi.u = load_any(src + D / 2);
+        float y[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x1 = (float)lo.h[e], x2 = (float)hi.h[e];
+            if (a.rotate && !is_v) {
+                const float2 w = cs[tok][8u * lane + e];
+                y[e] = fmaf(x1, w.x, -(x2 * w.y));
+                y[8 + e] = fmaf(x1, w.y, x2 * w.x);
+            } else {
+                y[e] = x1;
+                y[8 + e] = x2;
+            }
+            lo.h[e] = (h16)y[e];
+            hi.h[e] = (h16)y[8 + e];
+        }
+        uint16_t *rows_out = is_q ? a.q_out + (t0 + tok) * a.qos : is_v || a.k_out == nullptr ? nullptr : a.k_out + (t0 + tok) * a.kos;
+        if (rows_out != nullptr) {
+            store_any(rows_out + h * D + 8u * lane, lo.u);
+            store_any(rows_out + h * D + 8u * lane + D / 2, hi.u);
+        }
+        if (is_q || page_of[tok] < 0) continue;
+        const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u)); /* row of the page */
+        const uint64_t at = (uint64_t)page_of[tok] * a.kv.page_stride + (uint64_t)slot * D + 8u * lane;
+        if constexpr (!Q8) {
+            uint16_t *dst = (uint16_t *)(is_v ? a.kv.v : a.kv.k) + at;
+            *(uint4 *)dst = lo.u;
+            *(uint4 *)(dst + D / 2) = hi.u;
+        } else {
+            /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
+             * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8) */
+            float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m0 = fabsf(y[e]) < INFINITY ? fmaxf(m0, fabsf(y[e])) : INFINITY;
+                m1 = fabsf(y[8 + e]) < INFINITY ? fmaxf(m1, fabsf(y[8 + e])) : INFINITY;
+            }
+            if (D == 64) m0 = m1 = fmaxf(m0, m1); /* both halves are one group */
+#pragma unroll
+            for (u32 o = 1; o < LPR; o <<= 1) {
+                m0 = fmaxf(m0, __shfl_xor(m0, o));
+                m1 = fmaxf(m1, __shfl_xor(m1, o));
+            }
+            union {
+                int8_t b[8];
+                uint2 u;
+            } q0, q1;
+            const float s0 = m0 == 0.0f ? 1.0f : m0 / 127.0f, s1 = m1 == 0.0f ? 1.0f : m1 / 127.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                /* a group that is not finite: 0 times its NaN scale */
+                q0.b[e] = m0 < INFINITY ? (int8_t)fminf(fmaxf(rintf(y[e] / s0), -127.0f), 127.0f) : (int8_t)0;
+                q1.b[e] = m1 < INFINITY ? (int8_t)fminf(fmaxf(rintf(y[8 + e] / s1), -127.0f), 127.0f) : (int8_t)0;
+            }
+            int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
+            *(uint2 *)dst = q0.u;
+            *(uint2 *)(dst + D / 2) = q1.u;
+            if (lane == 0u) {
+                uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
+                sc[0] = m0 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
+                if (D == 128) sc[1] = m1 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
+            }
+        }
+    }
+}
+
+/* ---- gather ------------------------------------------------------------------- */
+
+/* A copy (Q8_0: fp16(q * scale)), bound by HBM: 8 or 16 values a lane, four
+ * items of a thread in flight. */
+template <int D, bool Q8>
+__global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb) {
+    constexpr u32 E = Q8 ? 16 : 8, LPR = D / E, U = 4;
+    const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
+    const u32 kvh = a.kv.heads, first = a.k_out == nullptr ? kvh : 0u, rows = (a.v_out == nullptr ? kvh : 2u * kvh) - first;
+    const u32 items = nt * rows * LPR;
+    for (u32 i0 = t; i0 < items; i0 += 256u * U) {
+        uint4 w[U];
+        u32 sc[U];
+#pragma unroll
+        for (u32 u = 0; u < U; ++u) {
+            const u32 i = i0 + 256u * u;
+            w[u] = make_uint4(0u, 0u, 0u, 0u);
+            sc[u] = 0u;
+            if (i >= items) continue;
+            const u32 lane = i % LPR, tok = t0 + i / LPR / rows, r = i / LPR % rows + first;
+            const int seq = a.seqs != nullptr ? a.seqs[tok] : (int)tok, pos = a.pos[tok];
+            if (seq < 0 || (u32)seq >= a.kv.n_seqs || pos < 0 || ((u32)pos >> a.kv.shift) >= a.kv.table_stride) continue;
+            const int page = kv_page(a.kv, seq, (u32)pos);
+            if (page < 0) continue;
+            const bool is_v = r >= kvh;
+            const u32 slot = ((is_v ? r - kvh : r) << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u));
+            const uint64_t at = (uint64_t)page * a.kv.page_stride + (uint64_t)slot * D + E * lane;
+            w[u] = *(const uint4 *)((const uint8_t *)(is_v ? a.kv.v : a.kv.k) + (Q8 ? at : 2u * at));
+            if (Q8) sc[u] = (is_v ? a.kv.vs : a.kv.ks)[(uint64_t)page * (a.kv.page_stride / 64u) + slot * (D / 64u) + lane / 4u];
+        }
+#pragma unroll
+        for (u32 u = 0; u < U; ++u) {
+            const u32 i = i0 + 256u * u;
+            if (i >= items) continue;
+            const u32 lane = i % LPR, tok = t0 + i / LPR / rows, r = i / LPR % rows + first;
+            uint16_t *dst = r >= kvh ? a.v_out + tok * a.vos + (r - kvh) * D : a.k_out + tok * a.kos + r * D;
+            if constexpr (!Q8) {
+                store_any(dst + 8u * lane, w[u]);
+            } else {
+                U4H8 lo, hi;
+                /* an absent token's zeros are zeros with any scale: its payload 0 and scale 0 */
+                lo.v = dequant_q8(w[u].x, w[u].y, sc[u]);
+                hi.v = dequant_q8(w[u].z, w[u].w, sc[u]);
+                store_any(dst + 16u * lane, lo.u);
+                store_any(dst + 16u * lane + 8u, hi.u);
+            }
+        }
+    }
+}
+
+/* ---- attention of one token ---------------------------------------------------- */
+
+constexpr u32 PA_TILE = 128;   /* tokens of a block's tile: 32 of each of its 4 wavefronts */
+constexpr u32 PA_BLOCKS = 512; /* 2 per CU: what the registers of a wavefront allow */
+
+struct PagedGrid {
+    uocr_paged_args a;
+    u32 group, chunks; /* query heads of a KV head; sets of up to 16 of them */
+    u32 rows;          /* of a partial: min(group, 16) */
+    float c;           /* scale * log2(e) */
+};
+
+__device__ const uint4 g_zero_row[16] = {};
+
+/* Tokens of sequence s, and the tiles of each of its head sets. */
+__device__ __forceinline__ u32 seq_len(const uocr_paged_args &a, u32 s) {
+    return (u32)min(max(a.lengths[s], 0), (int)(a.kv.table_stride << a.kv.shift));
+}
+__device__ __forceinline__ u32 len_tiles(u32 len) {
+    return max((len + PA_TILE - 1u) / PA_TILE, 1u); /* an empty sequence has its zeros to write */
+}
+
+/* The block's share of all tiles.  Tiles are numbered by sequence, head set and
+ * position; block b of G takes [N b / G, N (b + 1) / G), whatever sequences
+ * these belong to, so no length of one sequence leaves CUs idle. */
+__device__ __forceinline__ u32 busy_blocks(uint64_t n, u32 g) {
+    return n < g ? (u32)n : g; /* none without a tile */
+}
+__device__ __forceinline__ uint64_t share(uint64_t n, u32 b, u32 g) {
+    return n * b / g;
+}
+__device__ __forceinline__ u32 block_of(uint64_t n, uint64_t tile, u32 g) {
+    return (u32)(((tile + 1u) * g - 1u) / n);
+}
+
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
+    return ((uint64_t)(u32)__shfl_up((int)(v >> 32), d) << 32) | (u32)__shfl_up((int)v, d);
+}
+
+/* Prefix sums over the sequences' tiles, by the 256 threads of a block: every
+ * thread takes a run of sequences.  Returns the tiles before the thread's run
+ * and, in total, all tiles. */
+__device__ __forceinline__ uint64_t tiles_before(const PagedGrid &g, u32 run, uint64_t *total, uint64_t *red) {
+    const u32 t = threadIdx.x, sets = g.a.kv.heads * g.chunks;
+    uint64_t own = 0;
+    for (u32 s = t * run; s < min(t * run + run, g.a.kv.n_seqs); ++s) own += (uint64_t)len_tiles(seq_len(g.a, s)) * sets;
+    uint64_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t v = shfl_up64(sum, d);
+        if ((int)(t & 63u) >= d) sum += v;
+    }
+    if ((t & 63u) == 63u) red[t >> 6] = sum;
+    __syncthreads();
+    uint64_t before = sum - own, all = 0;
+#pragma unroll
+    for (u32 w = 0; w < 4; ++w) {
+        if (w < (t >> 6)) before += red[w];
+        all += red[w];
+    }
+    *total = all;
+    return before;
+}
+
+/* What a state with maximum m counts for beside one with maximum M >= m.  Only
+ * scores that are all NaN leave weight without a maximum: their NaN goes on. */
+__device__ __forceinline__ float state_factor(float m, float M, float c) {
+    return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c);
+}
+
+/* One pass over the cache with the running maximum and sum of the softmax.
+ * Bound by HBM on long caches and by the chain of dependent loads (lengths,
+ * page, rows) on short ones.
+ *
+ * The query heads of a KV head are one side of the MFMA tiles (up to 16; a
+ * group of one leaves 15 columns idle, which costs nothing: 16 MFMAs per 16 KB
+ * of cache are an eighth of what the CU could do meanwhile), so a cache row is
+ * read once for all of them.  A wavefront takes 32 tokens of the block's tile:
+ *   S^T = K Q^T, 16x16x32: lane l holds head l % 16 and tokens
+ *   16 n + 4 (l / 16) + i; K goes from memory straight into the operand (lane
+ *   l: token l % 16, 16 bytes at (l / 16));
+ *   O^T += V^T P^T: the probabilities stay where S^T left them, V goes through
+ *   LDS, row-major, and is transposed by the LDS read.
+ * Q8_0: K enters the MFMA as its integers (exact in fp16), a sum for each group
+ * of 64 dims, the fp32 sums times the scales; V as fp16(q * scale).
+ * Tokens past the length or in absent pages are read from a row of zeros: what
+ * stands there never enters a product.
+ *
+ * The wavefronts' states are merged in LDS; a head set that one block covers is
+ * written at once, else its fp32 state goes to the block's partials (at most
+ * two: its first and its last set) for k_paged_join. */
+template <int D, bool Q8>
+__global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
+    constexpr u32 ROW = D * (Q8 ? 1 : 2);      /* bytes of a cached row */
+    constexpr u32 NK = ROW / 64;               /* 16-byte loads of a lane per 16 keys */
+    constexpr u32 VL = ROW / 16;               /* lanes of a V row */
+    constexpr u32 NV = 32 * VL / 64;           /* V loads of a lane per 32 tokens */
+    constexpr u32 ORS = D + 4;                 /* floats from a head's row to the next, in LDS */
+    constexpr u32 WLDS = 16 * ORS * 4 > 64 * D ? 16 * ORS * 4 : 64 * D; /* V tile, later the state */
+    __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * WLDS];
+    __shared__ float sml[4][2][16];
+    __shared__ uint64_t red[4];
+    __shared__ u32 start_s;
+    __shared__ uint64_t start_n;
+    const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 15u, gr = lane >> 4;
+    const uocr_kv &kv = g.a.kv;
+    const u32 sets = kv.heads * g.chunks;
+
+    uint64_t total;
+    const u32 run = (kv.n_seqs + 255u) / 256u;
+    const uint64_t before = tiles_before(g, run, &total, red);
+    const u32 blocks = busy_blocks(total, gridDim.x);
+    if (blockIdx.x >= blocks) return;
+    const uint64_t lo = share(total, blockIdx.x, blocks), hi = share(total, blockIdx.x + 1u, blocks);
+    {
+        /* the thread whose run holds tile lo finds its sequence */
+        uint64_t n = before;
+        const u32 s1 = min(t * run + run, kv.n_seqs);
+        for (u32 s = t * run; s < s1; ++s) {
+            const uint64_t next = n + (uint64_t)len_tiles(seq_len(g.a, s)) * sets;
+            if (n <= lo && lo < next) {
+                start_s = s;
+                start_n = n;
+            }
+            n = next;
+        }
+    }
+    __syncthreads();
+    u32 s = start_s;
+    uint64_t base = start_n, at = lo;
+    uint8_t *vt = sm + wave * WLDS;
+    bool first = true;
+    while (at < hi) {
+        const u32 len = seq_len(g.a, s), nt = len_tiles(len);
+        if (at >= base + (uint64_t)nt * sets) {
+            base += (uint64_t)nt * sets;
+            ++s;
+            continue;
+        }
+        const u32 set = (u32)((at - base) / nt), ta = (u32)((at - base) % nt);
+        const u32 tb = (u32)min((uint64_t)nt, (uint64_t)ta + (hi - at)); /* the block's tiles of this set: [ta, tb) */
+        const u32 kvh = set / g.chunks, h0 = kvh * g.group + 16u * (set % g.chunks);
+        const u32 nh = min(16u, kvh * g.group + g.group - h0); /* query heads of the set */
+        const int32_t *table = kv.table + (uint64_t)s * kv.table_stride;
+
+        /* the query operand: head `col`, the dims that the K operand has in the same place */
+        U4H8 qr[D / 32];
+#pragma unroll
+        for (u32 x = 0; x < D / 32; ++x) {
+            const u32 d = Q8 ? 64u * (x / 2u) + 16u * gr + 8u * (x % 2u) : 32u * x + 8u * gr;
+            qr[x].u = make_uint4(0u, 0u, 0u, 0u);
+            if (col < nh) qr[x].u = load_any(g.a.q + (uint64_t)s * g.a.qs + (h0 + col) * D + d);
+        }
+        f32x4 o[D / 16];
+#pragma unroll
+        for (u32 n = 0; n < D / 16; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+
+        uint4 kr[2 * NK], vr[NV];
+        u32 ksc = 0, vsc = 0; /* scales of token lane % 32 */
+        u32 valid;            /* bit i: token i of the wavefront's 32 */
+        /* the page of token lane % 32 of the wavefront's part of tile x (-1: none) */
+        auto page = [&](u32 x) {
+            const u32 tok = x * PA_TILE + 32u * wave + (lane & 31u);
+            int p = -1;
+            if (x < tb && tok < len) {
+                p = table[tok >> kv.shift];
+                if ((u32)p >= kv.n_pages) p = -1;
+            }
+            return p;
+        };
+        auto load = [&](u32 x, int p) {
+            const u32 tok0 = x * PA_TILE + 32u * wave;
+            valid = (u32)__ballot(p >= 0);
+            const uint8_t *k = (const uint8_t *)kv.k, *v = (const uint8_t *)kv.v;
+            const u32 mask = (1u << kv.shift) - 1u, hrow = kvh << kv.shift;
+            auto row = [&](const uint8_t *pages, u32 i) {
+                const int pi = __shfl(p, (int)i);
+                const uint8_t *r = pages + ((uint64_t)(u32)pi * kv.page_stride + (uint64_t)(hrow + ((tok0 + i) & mask)) * D) * (Q8 ? 1u : 2u);
+                return pi >= 0 ? r : (const uint8_t *)g_zero_row;
+            };
+#pragma unroll
+            for (u32 n = 0; n < 2; ++n) {
+                const uint8_t *r = row(k, 16u * n + col) + 16u * gr;
+#pragma unroll
+                for (u32 x2 = 0; x2 < NK; ++x2) kr[n * NK + x2] = *(const uint4 *)(r + 64u * x2);
+            }
+#pragma unroll
+            for (u32 y = 0; y < NV; ++y) vr[y] = *(const uint4 *)(row(v, (64u / VL) * y + lane / VL) + 16u * (lane % VL));
+            if constexpr (Q8) {
+                ksc = vsc = 0u;
+                if (p >= 0) {
+                    const uint64_t sat = (uint64_t)(u32)p * (kv.page_stride / 64u) + (uint64_t)(hrow + ((tok0 + (lane & 31u)) & mask)) * (D / 64u);
+                    if (D == 128) {
+                        ksc = *(const u32 *)(kv.ks + sat);
+                        vsc = *(const u32 *)(kv.vs + sat);
+                    } else {
+                        ksc = kv.ks[sat];
+                        vsc = kv.vs[sat];
+                    }
+                }
+            }
+        };
+        load(ta, page(ta));
+        int pn = page(ta + 1u);
+        for (u32 x = ta; x < tb; ++x) {
+            const u32 now = valid;
+            float sc[8];
+            if (now != 0u) {
+                /* V to LDS, rows swizzled by pairs of 16-byte pieces so that the transposing reads touch all banks */
+                __builtin_amdgcn_wave_barrier();
+                auto swz = [](u32 key, u32 pc) { return key * (2u * D) + 16u * (pc ^ (D == 128 ? (key & 7u) << 1 : ((key >> 1) & 3u) << 1)); };
+#pragma unroll
+                for (u32 y = 0; y < NV; ++y) {
+                    const u32 key = (64u / VL) * y + lane / VL, pc = lane % VL;
+                    if constexpr (Q8) {
+                        const u32 s2 = (u32)__shfl((int)vsc, (int)key);
+                        const u32 sv = pc >= 4u ? s2 >> 16 : s2 & 0xffffu;
+                        U4H8 a, b;
+                        a.v = dequant_q8(vr[y].x, vr[y].y, sv);
+                        b.v = dequant_q8(vr[y].z, vr[y].w, sv);
+                        *(uint4 *)(vt + swz(key, 2u * pc)) = a.u;
+                        *(uint4 *)(vt + swz(key, 2u * pc + 1u)) = b.u;
+                    } else {
+                        *(uint4 *)(vt + swz(key, pc)) = vr[y];
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (u32 n = 0; n < 2; ++n) {
+                    if constexpr (Q8) {
+                        f32x4 part[D / 64];
+#pragma unroll
+                        for (u32 j = 0; j < D / 64; ++j) {
+                            part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                            part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].x, kr[n * NK + j].y, 0x3c00u), qr[2 * j].v, part[j], 0, 0, 0);
+                            part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].z, kr[n * NK + j].w, 0x3c00u), qr[2 * j + 1].v, part[j], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (u32 i = 0; i < 4; ++i) {
+                            const u32 s2 = (u32)__shfl((int)ksc, (int)(16u * n + 4u * gr + i));
+                            float v = part[0][i] * (float)__builtin_bit_cast(h16, (unsigned short)(s2 & 0xffffu));
+                            if (D == 128) v = fmaf(part[D / 64 - 1][i], (float)__builtin_bit_cast(h16, (unsigned short)(s2 >> 16)), v);
+                            sc[4 * n + i] = v;
+                        }
+                    } else {
+                        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (u32 x2 = 0; x2 < NK; ++x2) {
+                            U4H8 kk;
+                            kk.u = kr[n * NK + x2];
+                            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk.v, qr[x2].v, a, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (u32 i = 0; i < 4; ++i) sc[4 * n + i] = a[i];
+                    }
+                }
+            }
+            if (x + 1u < tb) {
+                load(x + 1u, pn);
+                pn = page(x + 2u);
+            }
+            if (now == 0u) continue;
+            if (now != 0xffffffffu) {
+#pragma unroll
+                for (u32 i = 0; i < 8; ++i)
+                    if (!((now >> (16u * (i / 4u) + 4u * gr + i % 4u)) & 1u)) sc[i] = -INFINITY;
+            }
+            float tm = sc[0];
+#pragma unroll
+            for (u32 i = 1; i < 8; ++i) tm = fmaxf(tm, sc[i]);
+            tm = fmaxf(tm, __shfl_xor(tm, 16));
+            tm = fmaxf(tm, __shfl_xor(tm, 32));
+            if (__any(tm > m)) {
+                const float mn = fmaxf(m, tm), corr = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * g.c);
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (u32 n = 0; n < D / 16; ++n)
+#pragma unroll
+                    for (u32 i = 0; i < 4; ++i) o[n][i] *= corr;
+            }
+            const float mc = m == -INFINITY ? 0.0f : m * g.c;
+            U4H8 p;
+#pragma unroll
+            for (u32 i = 0; i < 8; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -mc));
+                l += e;
+                p.h[i] = (h16)e;
+            }
+#pragma unroll
+            for (u32 n = 0; n < D / 16; ++n) {
+                /* the lane's key of the transposing read: 4 gr + lane / 4 % 4 (and + 16), its dims 16 n + 4 (lane % 4) */
+                const u32 key = 4u * gr + ((lane >> 2) & 3u);
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                auto tr = [&](u32 kk) {
+                    const u32 pc = 2u * n + ((lane >> 1) & 1u);
+                    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4 *)(vt + kk * (2u * D) + 16u * (pc ^ (D == 128 ? (kk & 7u) << 1 : ((kk >> 1) & 3u) << 1)) + 8u * (lane & 1u))));
+                };
+                const uint2 a0 = tr(key), a1 = tr(key + 16u);
+                U4H8 vv;
+                vv.u = make_uint4(a0.x, a0.y, a1.x, a1.y);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv.v, p.v, o[n], 0, 0, 0);
+            }
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        /* the four states: lane holds head col, dims 16 n + 4 gr + i */
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (u32 n = 0; n < D / 16; ++n) *(f32x4 *)(vt + (col * ORS + 16u * n + 4u * gr) * 4u) = o[n];
+        if (lane < 16u) {
+            sml[wave][0][col] = m;
+            sml[wave][1][col] = l;
+        }
+        __syncthreads();
+        const bool whole = ta == 0u && tb == nt;
+        const u32 slot = 2u * blockIdx.x + (first ? 0u : 1u);
+        for (u32 i = t; i < nh * (D / 4); i += 256u) {
+            const u32 h = i / (D / 4), d = 4u * (i % (D / 4));
+            const float M = fmaxf(fmaxf(sml[0][0][h], sml[1][0][h]), fmaxf(sml[2][0][h], sml[3][0][h]));
+            float L = 0.0f;
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (u32 w = 0; w < 4; ++w) {
+                const float mw = sml[w][0][h], lw = sml[w][1][h];
+                const f32x4 x = *(const f32x4 *)(sm + w * WLDS + (h * ORS + d) * 4u);
+                if (lw == 0.0f) continue; /* no weight in this wavefront's tokens */
+                const float f = state_factor(mw, M, g.c);
+                L = fmaf(lw, f, L);
+#pragma unroll
+                for (u32 e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+            }
+            if (whole) {
+                const float li = L == 0.0f ? 0.0f : 1.0f / L;
+                uint16_t *dst = g.a.out + (uint64_t)s * g.a.os + (h0 + h) * D + d;
+#pragma unroll
+                for (u32 e = 0; e < 4; ++e) dst[e] = __builtin_bit_cast(uint16_t, (h16)(v[e] * li));
+            } else {
+                float *part = g.a.part + (uint64_t)slot * g.rows * (D + 4);
+                *(f32x4 *)(part + h * (D + 4) + d) = v;
+                if (d == 0u) *(float2 *)(part + h * (D + 4) + D) = make_float2(M, L);
+            }
+        }
+        __syncthreads();
+        at += tb - ta;
+        first = false;
+    }
+}
+
+/* Joins the partials of a head that several blocks had tiles of:
+ * out = sum_b o_b 2^((m_b - M) c) / sum_b l_b 2^((m_b - M) c).  A block for
+ * each sequence and head; 256 / (D / 4) partials are read at a time. */
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_join(PagedGrid g, u32 grid) {
+    constexpr u32 LN = D / 4, PAR = 256 / LN;
+    __shared__ uint64_t red[4], before_s;
+    __shared__ float wm[4];
+    __shared__ f32x4 acc[PAR][LN];
+    __shared__ float lsum[PAR];
+    const u32 t = threadIdx.x, s = blockIdx.x / g.a.hq, h = blockIdx.x % g.a.hq;
+    const uocr_kv &kv = g.a.kv;
+    const u32 kvh = h / g.group, set = kvh * g.chunks + h % g.group / 16u, row = h % g.group % 16u, sets = kv.heads * g.chunks;
+    const u32 nt = len_tiles(seq_len(g.a, s));
+    uint64_t total;
+    const u32 run = (kv.n_seqs + 255u) / 256u;
+    uint64_t before = tiles_before(g, run, &total, red);
+    if (s / run == t) {
+        for (u32 i = t * run; i < s; ++i) before += (uint64_t)len_tiles(seq_len(g.a, i)) * sets;
+        before_s = before;
+    }
+    __syncthreads();
+    const u32 blocks = busy_blocks(total, grid);
+    const uint64_t T0 = before_s + (uint64_t)set * nt;
+    const u32 b0 = block_of(total, T0, blocks), b1 = block_of(total, T0 + nt - 1u, blocks);
+    if (b0 == b1) return; /* one block had all of it */
+    auto part = [&](u32 b) { /* the set is the block's first unless the block began before it */
+        return g.a.part + ((uint64_t)(2u * b + (share(total, b, blocks) >= T0 ? 0u : 1u)) * g.rows + row) * (D + 4);
+    };
+    float M = -INFINITY;
+    for (u32 b = b0 + t; b <= b1; b += 256u) M = fmaxf(M, part(b)[D]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    if ((t & 63u) == 0u) wm[t >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    const u32 ln = t % LN, p = t / LN;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    float L = 0.0f;
+    for (u32 b = b0 + p; b <= b1; b += PAR) {
+        const float *x = part(b);
+        const float2 ml = *(const float2 *)(x + D);
+        const f32x4 o = *(const f32x4 *)(x + 4u * ln);
+        if (ml.y == 0.0f) continue; /* no weight there */
+        const float f = state_factor(ml.x, M, g.c);
+        L = fmaf(ml.y, f, L);
+#pragma unroll
+        for (u32 e = 0; e < 4; ++e) v[e] = fmaf(o[e], f, v[e]);
+    }
+    acc[p][ln] = v;
+    if (ln == 0u) lsum[p] = L;
+    __syncthreads();
+    if (t < LN) {
+        L = lsum[0];
+#pragma unroll
+        for (u32 x = 1; x < PAR; ++x) {
+            L += lsum[x];
+            const f32x4 o = acc[x][t];
+#pragma unroll
+            for (u32 e = 0; e < 4; ++e) v[e] += o[e];
+        }
+        const float li = L == 0.0f ? 0.0f : 1.0f / L;
+        uint16_t *dst = g.a.out + (uint64_t)s * g.a.os + h * D + 4u * t;
+#pragma unroll
+        for (u32 e = 0; e < 4; ++e) dst[e] = __builtin_bit_cast(uint16_t, (h16)(v[e] * li));
+    }
+}
+
+}  // namespace
+
+hipError_t uocr_launch_kv_append(hipStream_t st, const uocr_append_args *a) {
+    /* a block for at least 256 lanes' work, so that few heads do not leave most of it idle */
+    const u32 lanes = (a->heads + 2u * a->kv.heads) * (a->kv.dim / 16u);
+    const u32 tpb = lanes >= 256u ? 1u : (256u / lanes < APPEND_TOKENS ? 256u / lanes : APPEND_TOKENS);
+    const dim3 grid((a->tokens + tpb - 1u) / tpb);
+    if (a->kv.dim == 128u) {
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_append<128, true>), grid, dim3(256), 0, st, *a, tpb);
+        else hipLaunchKernelGGL((k_kv_append<128, false>), grid, dim3(256), 0, st, *a, tpb);
+    } else {
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_append<64, true>), grid, dim3(256), 0, st, *a, tpb);
+        else hipLaunchKernelGGL((k_kv_append<64, false>), grid, dim3(256), 0, st, *a, tpb);
+    }
+    return hipGetLastError();
+}
+
+hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
+    const u32 sides = (a->k_out != nullptr ? 1u : 0u) + (a->v_out != nullptr ? 1u : 0u);
+    const u32 lanes = sides * a->kv.heads * a->kv.dim / (a->kv.q8 ? 16u : 8u);
+    const u32 tpb = lanes >= 1024u ? 1u : 1024u / lanes; /* 1,024 items: four of each thread */
+    const dim3 grid((a->tokens + tpb - 1u) / tpb);
+    if (a->kv.dim == 128u) {
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<128, true>), grid, dim3(256), 0, st, *a, tpb);
+        else hipLaunchKernelGGL((k_kv_gather<128, false>), grid, dim3(256), 0, st, *a, tpb);
+    } else {
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<64, true>), grid, dim3(256), 0, st, *a, tpb);
+        else hipLaunchKernelGGL((k_kv_gather<64, false>), grid, dim3(256), 0, st, *a, tpb);
+    }
+    return hipGetLastError();
+}
+
+size_t uocr_paged_attention_ws_bytes(uint32_t heads, uint32_t kv_heads, uint32_t dim) {
+    const u32 group = heads / kv_heads, rows = group < 16u ? group : 16u;
+    return (size_t)2u * PA_BLOCKS * rows * (dim + 4u) * sizeof(float);
+}
+
+hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a) {
+    PagedGrid g;
+    g.a = *a;
+    g.group = a->hq / a->kv.heads;
+    g.chunks = (g.group + 15u) / 16u;
+    g.rows = g.group < 16u ? g.group : 16u;
+    g.c = a->scale * 1.4426950408889634f;
+    const uint64_t most = ((uint64_t)(a->kv.table_stride << a->kv.shift) + PA_TILE - 1u) / PA_TILE; /* tiles of a set */
+    const uint64_t tiles = most * a->kv.n_seqs * a->kv.heads * g.chunks;
+    const u32 blocks = tiles < PA_BLOCKS ? (u32)tiles : PA_BLOCKS;
+    if (a->kv.dim == 128u) {
+        if (a->kv.q8) hipLaunchKernelGGL((k_paged_attention<128, true>), dim3(blocks), dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((k_paged_attention<128, false>), dim3(blocks), dim3(256), 0, st, g);
+    } else {
+        if (a->kv.q8) hipLaunchKernelGGL((k_paged_attention<64, true>), dim3(blocks), dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((k_paged_attention<64, false>), dim3(blocks), dim3(256), 0, st, g);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || most == 1u) return e; /* one tile a set: nothing to join */
+    const dim3 grid(a->kv.n_seqs * a->hq);
+    if (a->kv.dim == 128u) hipLaunchKernelGGL((k_paged_join<128>), grid, dim3(256), 0, st, g, blocks);
+    else hipLaunchKernelGGL((k_paged_join<64>), grid, dim3(256), 0, st, g, blocks);
+    return hipGetLastError();
+}

@@ -12,6 +12,7 @@
 
 #include "uocr_hip.h"
 #include "uocr_kernels.h"
+#include "uocr_serve.h"
 
 namespace {
 
@@ -613,6 +614,292 @@ extern "C" int uocr_op_moe_ffn_rows_static(const uocr_op_moe_weights *m, const v
         return op_fail(UOCR_ERROR_INTERNAL, "static scratch address unavailable: %s", hipGetErrorString(g_scratch_err));
     }
     return moe_rows(st, m, x, norm_w, residual, rows, norm_topk, g_scratch_dev, out);
+}
+
+/* ---- serving several sequences ------------------------------------------------ */
+
+namespace {
+
+/* The operator stream belongs to device 0: the launches below are made with it
+ * current, and the caller's device is put back. */
+struct on_device0 {
+    int before = 0;
+    on_device0() {
+        if (hipGetDevice(&before) == hipSuccess && before != 0) (void)hipSetDevice(0);
+    }
+    ~on_device0() {
+        if (before != 0) (void)hipSetDevice(before);
+    }
+};
+
+bool off(const void *p, uintptr_t to) {
+    return ((uintptr_t)p & (to - 1u)) != 0u;
+}
+
+/* The checked form of a cache; an error leaves its text. */
+int pages_of(const uocr_op_kv_pages *c, const char *what, uocr_kv *kv) {
+    if (c == nullptr || c->k == nullptr || c->v == nullptr || c->page_table == nullptr) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: the cache has no k, v or page_table", what);
+    }
+    if (c->qtype != UOCR_QT_F16 && c->qtype != UOCR_QT_Q8) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: pages are fp16 (1) or Q8_0 (3), not type %u", what, c->qtype);
+    }
+    if (c->head_dim != 64u && c->head_dim != 128u) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: head_dim is 64 or 128, not %u", what, c->head_dim);
+    }
+    if (c->kv_heads == 0u || c->kv_heads > UOCR_SERVE_MAX_HEADS || c->n_seqs == 0u || c->n_seqs > UOCR_SERVE_MAX_SEQS ||
+        c->n_pages == 0u || c->n_pages > 0x7fffffffu || c->table_stride == 0u || c->reserved0 != 0u) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "%s: kv_heads 1 to %u, n_seqs 1 to %u, n_pages below 2^31, table_stride from 1, reserved0 0", what,
+                       UOCR_SERVE_MAX_HEADS, UOCR_SERVE_MAX_SEQS);
+    }
+    const uint32_t page = c->page_tokens;
+    if (page == 0u || page > 65536u || (page & (page - 1u)) != 0u || (uint64_t)c->table_stride * page > 0x7fffffffu) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "%s: page_tokens is a power of two up to 65536 and table_stride * page_tokens below 2^31", what);
+    }
+    const uint64_t dense = (uint64_t)c->kv_heads * page * c->head_dim;
+    const uint64_t stride = c->page_stride != 0u ? c->page_stride : dense;
+    if (stride < dense || stride % c->head_dim != 0u || stride > (1ull << 40)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: page_stride is a multiple of head_dim of at least a page", what);
+    }
+    if (off(c->k, 16) || off(c->v, 16) || off(c->page_table, 4)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: k and v stand on 16-byte boundaries, the table on 4", what);
+    }
+    if (c->qtype == UOCR_QT_Q8 && (c->k_scales == nullptr || c->v_scales == nullptr || off(c->k_scales, 4) || off(c->v_scales, 4))) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: Q8_0 pages have k_scales and v_scales on 4-byte boundaries", what);
+    }
+    kv->k = c->k;
+    kv->v = c->v;
+    kv->ks = (uint16_t *)c->k_scales;
+    kv->vs = (uint16_t *)c->v_scales;
+    kv->table = c->page_table;
+    kv->page_stride = stride;
+    kv->table_stride = c->table_stride;
+    kv->n_pages = c->n_pages;
+    kv->n_seqs = c->n_seqs;
+    kv->heads = c->kv_heads;
+    kv->shift = (uint32_t)__builtin_ctz(page);
+    kv->dim = c->head_dim;
+    kv->q8 = c->qtype == UOCR_QT_Q8;
+    return UOCR_OK;
+}
+
+/* Rows of `heads` heads at p, `stride` values apart. */
+bool rows_ok(const void *p, uint64_t stride, uint64_t heads, uint64_t dim) {
+    return p != nullptr && !off(p, 2) && stride >= heads * dim && stride <= (1ull << 40);
+}
+
+bool scale_ok(float scale) {
+    return scale >= 0.0f && scale <= 1.8446744e19f; /* false for NaN; scores stay finite in fp32 */
+}
+
+}  // namespace
+
+extern "C" int uocr_op_kv_append(const uocr_op_kv_pages *pages, uint32_t tokens, const int32_t *seqs,
+                                 const int32_t *positions, uint32_t heads, float rope_theta, const void *q,
+                                 uint64_t q_stride, void *q_out, uint64_t q_out_stride, const void *k,
+                                 uint64_t k_stride, void *k_out, uint64_t k_out_stride, const void *v,
+                                 uint64_t v_stride) {
+    uocr_append_args a;
+    memset(&a, 0, sizeof(a));
+    const int r = pages_of(pages, "kv_append", &a.kv);
+    if (r != UOCR_OK) return r;
+    const uint32_t kvh = a.kv.heads, dim = a.kv.dim;
+    if (tokens > 0x7fffffffu || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
+        (seqs == nullptr && tokens > a.kv.n_seqs)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: positions, and a sequence for each token, are needed");
+    }
+    if (q != nullptr ? heads == 0u || heads > UOCR_SERVE_MAX_HEADS || !rows_ok(q, q_stride, heads, dim) ||
+                           !rows_ok(q_out, q_out_stride, heads, dim) || (q_out == q && q_out_stride != q_stride)
+                     : q_out != nullptr) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "kv_append: q and q_out come together, heads 1 to %u, rows at least heads * head_dim apart", UOCR_SERVE_MAX_HEADS);
+    }
+    if (!rows_ok(k, k_stride, kvh, dim) || !rows_ok(v, v_stride, kvh, dim) ||
+        (k_out != nullptr && (!rows_ok(k_out, k_out_stride, kvh, dim) || (k_out == k && k_out_stride != k_stride)))) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: k and v rows are at least kv_heads * head_dim apart");
+    }
+    if (!(rope_theta >= 0.0f && rope_theta <= 3.0e38f)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: rope_theta is positive, or 0 for no rotation");
+    }
+    STREAM_OR_RETURN(st);
+    if (tokens == 0u) return UOCR_OK;
+    const on_device0 dev;
+    a.seqs = seqs;
+    a.pos = positions;
+    a.tokens = tokens;
+    a.heads = q != nullptr ? heads : 0u;
+    a.log2_theta = rope_theta > 0.0f ? log2((double)rope_theta) : 0.0;
+    a.rotate = rope_theta > 0.0f;
+    a.q = (const uint16_t *)q;
+    a.k = (const uint16_t *)k;
+    a.v = (const uint16_t *)v;
+    a.q_out = (uint16_t *)q_out;
+    a.k_out = (uint16_t *)k_out;
+    a.qs = q_stride;
+    a.ks = k_stride;
+    a.vs = v_stride;
+    a.qos = q_out_stride;
+    a.kos = k_out_stride;
+    return hip_status(uocr_launch_kv_append(st, &a), "kv_append");
+}
+
+extern "C" int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens, const int32_t *seqs,
+                                 const int32_t *positions, void *k_out, uint64_t k_out_stride, void *v_out,
+                                 uint64_t v_out_stride) {
+    uocr_gather_args a;
+    memset(&a, 0, sizeof(a));
+    const int r = pages_of(pages, "kv_gather", &a.kv);
+    if (r != UOCR_OK) return r;
+    if (tokens > 0x7fffffffu || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
+        (seqs == nullptr && tokens > a.kv.n_seqs)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_gather: positions, and a sequence for each token, are needed");
+    }
+    if ((k_out == nullptr && v_out == nullptr) ||
+        (k_out != nullptr && !rows_ok(k_out, k_out_stride, a.kv.heads, a.kv.dim)) ||
+        (v_out != nullptr && !rows_ok(v_out, v_out_stride, a.kv.heads, a.kv.dim))) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_gather: k_out or v_out, rows at least kv_heads * head_dim apart");
+    }
+    STREAM_OR_RETURN(st);
+    if (tokens == 0u) return UOCR_OK;
+    const on_device0 dev;
+    a.seqs = seqs;
+    a.pos = positions;
+    a.tokens = tokens;
+    a.k_out = (uint16_t *)k_out;
+    a.v_out = (uint16_t *)v_out;
+    a.kos = k_out_stride;
+    a.vos = v_out_stride;
+    return hip_status(uocr_launch_kv_gather(st, &a), "kv_gather");
+}
+
+extern "C" size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads,
+                                                          uint32_t head_dim) {
+    if (n_seqs == 0u || n_seqs > UOCR_SERVE_MAX_SEQS || kv_heads == 0u || heads == 0u || heads > UOCR_SERVE_MAX_HEADS ||
+        heads % kv_heads != 0u || (head_dim != 64u && head_dim != 128u)) {
+        return 0u;
+    }
+    return uocr_paged_attention_ws_bytes(heads, kv_heads, head_dim);
+}
+
+extern "C" int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_t *lengths, uint32_t heads,
+                                       float scale, const void *q, uint64_t q_stride, void *workspace, void *out,
+                                       uint64_t out_stride) {
+    uocr_paged_args a;
+    memset(&a, 0, sizeof(a));
+    const int r = pages_of(pages, "paged_attention", &a.kv);
+    if (r != UOCR_OK) return r;
+    if (heads == 0u || heads > UOCR_SERVE_MAX_HEADS || heads % a.kv.heads != 0u) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "paged_attention: heads is a multiple of kv_heads up to %u", UOCR_SERVE_MAX_HEADS);
+    }
+    if (lengths == nullptr || off(lengths, 4) || workspace == nullptr || off(workspace, 16) || !scale_ok(scale) ||
+        !rows_ok(q, q_stride, heads, a.kv.dim) || !rows_ok(out, out_stride, heads, a.kv.dim) ||
+        (out == q && out_stride != q_stride)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "paged_attention: lengths, a workspace on 16 bytes, a scale from 0 and rows at least heads * head_dim apart are needed");
+    }
+    STREAM_OR_RETURN(st);
+    const on_device0 dev;
+    a.lengths = lengths;
+    a.hq = heads;
+    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)a.kv.dim);
+    a.q = (const uint16_t *)q;
+    a.out = (uint16_t *)out;
+    a.qs = q_stride;
+    a.os = out_stride;
+    a.part = (float *)workspace;
+    return hip_status(uocr_launch_paged_attention(st, &a), "paged_attention");
+}
+
+extern "C" int uocr_op_packed_attention(uint32_t n_seqs, const int32_t *q_starts, uint32_t q_tokens,
+                                        const int32_t *k_starts, uint32_t k_tokens, uint32_t heads, uint32_t kv_heads,
+                                        uint32_t head_dim, float scale, const void *q, uint64_t q_stride, const void *k,
+                                        uint64_t k_stride, const void *v, uint64_t v_stride, void *out,
+                                        uint64_t out_stride) {
+    if (n_seqs == 0u || n_seqs > UOCR_SERVE_MAX_SEQS || q_starts == nullptr || off(q_starts, 4) ||
+        (k_starts != nullptr && off(k_starts, 4)) || q_tokens > 0x7fffffffu || k_tokens > 0x7fffffffu ||
+        (k_starts == nullptr && k_tokens != q_tokens)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "packed_attention: n_seqs 1 to %u, starts, tokens below 2^31 (without k_starts as many keys as queries)", UOCR_SERVE_MAX_SEQS);
+    }
+    if ((head_dim != 64u && head_dim != 128u) || kv_heads == 0u || heads == 0u || heads > UOCR_SERVE_MAX_HEADS ||
+        heads % kv_heads != 0u || !scale_ok(scale)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
+                       "packed_attention: head_dim 64 or 128, heads a multiple of kv_heads up to %u, scale from 0", UOCR_SERVE_MAX_HEADS);
+    }
+    if (q_tokens != 0u && (!rows_ok(q, q_stride, heads, head_dim) || !rows_ok(out, out_stride, heads, head_dim) ||
+                           (out == q && out_stride != q_stride))) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "packed_attention: q and out rows are at least heads * head_dim apart");
+    }
+    if (k_tokens != 0u && (!rows_ok(k, k_stride, kv_heads, head_dim) || !rows_ok(v, v_stride, kv_heads, head_dim) ||
+                           k_stride >= (1u << 22) || v_stride >= (1u << 22))) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "packed_attention: k and v rows are kv_heads * head_dim to 2^22 values apart");
+    }
+    STREAM_OR_RETURN(st);
+    if (q_tokens == 0u) return UOCR_OK;
+    const on_device0 dev;
+    uocr_packed_args a;
+    memset(&a, 0, sizeof(a));
+    a.q_starts = q_starts;
+    a.k_starts = k_starts != nullptr ? k_starts : q_starts;
+    a.n_seqs = n_seqs;
+    a.q_tokens = q_tokens;
+    a.k_tokens = k_tokens;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.dim = head_dim;
+    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
+    a.q = (const uint16_t *)q;
+    a.k = (const uint16_t *)k;
+    a.v = (const uint16_t *)v;
+    a.out = (uint16_t *)out;
+    a.qs = q_stride;
+    a.ks = k_stride;
+    a.vs = v_stride;
+    a.os = out_stride;
+    return hip_status(uocr_launch_packed_attention(st, &a), "packed_attention");
+}
+
+extern "C" size_t uocr_op_sample_workspace_bytes(uint32_t rows, uint32_t vocab) {
+    return uocr_sample_ws_bytes(rows, vocab);
+}
+
+extern "C" int uocr_op_sample(uint32_t type, uint32_t rows, uint32_t vocab, const void *logits, uint64_t stride,
+                              const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                              const float *uniform, void *workspace, int32_t *tokens, float *probs) {
+    const uintptr_t size = type == UOCR_TENSOR_F32 ? 4u : 2u;
+    if (type != UOCR_QT_F16 && type != UOCR_TENSOR_F32) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "sample: logits are fp16 (1) or fp32 (2), not type %u", type);
+    }
+    if (vocab == 0u || vocab > (1u << 24) || rows > UOCR_SERVE_MAX_SEQS || logits == nullptr || off(logits, size) ||
+        stride < vocab || stride > (1ull << 40)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "sample: vocab 1 to 2^24, rows up to %u, rows of logits at least vocab apart",
+                       UOCR_SERVE_MAX_SEQS);
+    }
+    if (uniform == nullptr || workspace == nullptr || off(workspace, 16) || tokens == nullptr || off(tokens, 4) ||
+        off(uniform, 4) || off(temperature, 4) || off(top_k, 4) || off(top_p, 4) || off(min_p, 4) || off(probs, 4)) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "sample: uniform, tokens and a workspace on 16 bytes are needed");
+    }
+    STREAM_OR_RETURN(st);
+    if (rows == 0u) return UOCR_OK;
+    const on_device0 dev;
+    uocr_sample_args a;
+    memset(&a, 0, sizeof(a));
+    a.logits = logits;
+    a.stride = stride;
+    a.f32 = type == UOCR_TENSOR_F32;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.temperature = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.uniform = uniform;
+    a.ws = workspace;
+    a.tokens = tokens;
+    a.probs = probs;
+    return hip_status(uocr_launch_sample(st, &a), "sample");
 }
 
 /* ---- plumbing -------------------------------------------------------------- */

@@ -34,7 +34,7 @@ UOCR_ERROR_INTERNAL = -5
 UOCR_MEMORY_CATEGORY_COUNT = 10
 UOCR_PROFILE_MAX_EVENTS = 256
 
-QT_F16, QT_Q8, QT_Q4 = 1, 3, 4
+QT_F16, QT_F32, QT_Q8, QT_Q4 = 1, 2, 3, 4
 QPROFILE_FP16, QPROFILE_Q8, QPROFILE_Q4 = 1, 2, 3
 GEN_IGNORE_EOS, GEN_NO_GRAPH, GEN_TOKEN_PREFILL, GEN_NO_RUN = 1, 2, 4, 8
 
@@ -99,6 +99,15 @@ class CMoeWeights(ct.Structure):
                 ("sdown_w", ct.c_void_p), ("sdown_s", ct.c_void_p)]
 
 
+class CKvPages(ct.Structure):
+    """uocr_op_kv_pages: a paged KV cache (device addresses as integers)."""
+    _fields_ = [("qtype", ct.c_uint32), ("kv_heads", ct.c_uint32), ("head_dim", ct.c_uint32),
+                ("page_tokens", ct.c_uint32), ("n_pages", ct.c_uint32), ("n_seqs", ct.c_uint32),
+                ("table_stride", ct.c_uint32), ("reserved0", ct.c_uint32), ("page_stride", ct.c_uint64),
+                ("k", ct.c_void_p), ("v", ct.c_void_p), ("k_scales", ct.c_void_p), ("v_scales", ct.c_void_p),
+                ("page_table", ct.c_void_p)]
+
+
 # Exported symbols of include/unlimitedocr.h, include/uocr_hip.h and
 # include/uocr_synth.h: name -> (argtypes, restype).
 _VP, _U32, _I32, _SZ = ct.c_void_p, ct.c_uint32, ct.c_int32, ct.c_size_t
@@ -146,6 +155,16 @@ SIGNATURES = {
     "uocr_op_moe_rows_workspace_bytes": ([_U32], _SZ),
     "uocr_op_moe_ffn_rows": ([ct.POINTER(CMoeWeights), _VP, _VP, _VP, _U32, ct.c_int, _VP, _VP], ct.c_int),
     "uocr_op_moe_ffn_rows_static": ([ct.POINTER(CMoeWeights), _VP, _VP, _VP, _U32, ct.c_int, _VP], ct.c_int),
+    "uocr_op_kv_append": ([ct.POINTER(CKvPages), _U32, _VP, _VP, _U32, ct.c_float, _VP, ct.c_uint64, _VP, ct.c_uint64,
+                           _VP, ct.c_uint64, _VP, ct.c_uint64, _VP, ct.c_uint64], ct.c_int),
+    "uocr_op_kv_gather": ([ct.POINTER(CKvPages), _U32, _VP, _VP, _VP, ct.c_uint64, _VP, ct.c_uint64], ct.c_int),
+    "uocr_op_paged_attention_workspace_bytes": ([_U32, _U32, _U32, _U32], _SZ),
+    "uocr_op_paged_attention": ([ct.POINTER(CKvPages), _VP, _U32, ct.c_float, _VP, ct.c_uint64, _VP, _VP, ct.c_uint64],
+                                ct.c_int),
+    "uocr_op_packed_attention": ([_U32, _VP, _U32, _VP, _U32, _U32, _U32, _U32, ct.c_float, _VP, ct.c_uint64, _VP,
+                                  ct.c_uint64, _VP, ct.c_uint64, _VP, ct.c_uint64], ct.c_int),
+    "uocr_op_sample_workspace_bytes": ([_U32, _U32], _SZ),
+    "uocr_op_sample": ([_U32, _U32, _U32, _VP, ct.c_uint64, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP], ct.c_int),
     "uocr_hip_device_count": ([], ct.c_int),
     "uocr_hip_alloc": ([_SZ], _VP),
     "uocr_hip_free": ([_VP], ct.c_int),
@@ -603,6 +622,50 @@ def op_moe_ffn_rows_static(weights: CMoeWeights, x, norm_w, residual, rows, norm
     device allocation; rows <= STATIC_MAX_ROWS)."""
     _check_op(load_library().uocr_op_moe_ffn_rows_static(ct.byref(weights), _p(x), _p(norm_w), _p(residual), rows,
                                                          norm_topk, _p(out)), "op_moe_ffn_rows_static")
+
+
+def op_kv_append(pages: CKvPages, tokens, seqs, positions, heads, rope_theta, q, q_stride, q_out, q_out_stride, k,
+                 k_stride, k_out, k_out_stride, v, v_stride) -> None:
+    """Rotate the queries and keys of new tokens and write keys and values into their pages."""
+    _check_op(load_library().uocr_op_kv_append(ct.byref(pages), tokens, _p(seqs), _p(positions), heads, rope_theta,
+                                               _p(q), q_stride, _p(q_out), q_out_stride, _p(k), k_stride, _p(k_out),
+                                               k_out_stride, _p(v), v_stride), "op_kv_append")
+
+
+def op_kv_gather(pages: CKvPages, tokens, seqs, positions, k_out, k_out_stride, v_out, v_out_stride) -> None:
+    """Cached tokens as fp16 rows."""
+    _check_op(load_library().uocr_op_kv_gather(ct.byref(pages), tokens, _p(seqs), _p(positions), _p(k_out),
+                                               k_out_stride, _p(v_out), v_out_stride), "op_kv_gather")
+
+
+def paged_attention_workspace_bytes(n_seqs, heads, kv_heads, head_dim) -> int:
+    return load_library().uocr_op_paged_attention_workspace_bytes(n_seqs, heads, kv_heads, head_dim)
+
+
+def op_paged_attention(pages: CKvPages, lengths, heads, scale, q, q_stride, ws, out, out_stride) -> None:
+    """Attention of one new token of each sequence over its pages (scale 0: 1 / sqrt(head_dim))."""
+    _check_op(load_library().uocr_op_paged_attention(ct.byref(pages), _p(lengths), heads, scale, _p(q), q_stride,
+                                                     _p(ws), _p(out), out_stride), "op_paged_attention")
+
+
+def op_packed_attention(n_seqs, q_starts, q_tokens, k_starts, k_tokens, heads, kv_heads, head_dim, scale, q, q_stride,
+                        k, k_stride, v, v_stride, out, out_stride) -> None:
+    """Causal attention of prompts packed behind each other; each prompt's queries are the last of its keys."""
+    _check_op(load_library().uocr_op_packed_attention(n_seqs, _p(q_starts), q_tokens, _p(k_starts), k_tokens, heads,
+                                                      kv_heads, head_dim, scale, _p(q), q_stride, _p(k), k_stride,
+                                                      _p(v), v_stride, _p(out), out_stride), "op_packed_attention")
+
+
+def sample_workspace_bytes(rows, vocab) -> int:
+    return load_library().uocr_op_sample_workspace_bytes(rows, vocab)
+
+
+def op_sample(logits_type, rows, vocab, logits, stride, temperature, top_k, top_p, min_p, uniform, ws, tokens,
+              probs=None) -> None:
+    """A token of each row of logits by the row's settings and its uniform number."""
+    _check_op(load_library().uocr_op_sample(logits_type, rows, vocab, _p(logits), stride, _p(temperature), _p(top_k),
+                                            _p(top_p), _p(min_p), _p(uniform), _p(ws), _p(tokens), _p(probs)),
+              "op_sample")
 
 
 class Timer:
