@@ -361,8 +361,10 @@ UOCR_API int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens, c
                                const int32_t *positions, void *k_out, uint64_t k_out_stride, void *v_out,
                                uint64_t v_out_stride);
 
-/* Bytes of uocr_op_paged_attention's workspace (any contents), or 0 for sizes
- * that it refuses. */
+/* Bytes of uocr_op_paged_attention's workspace, or 0 for sizes that it refuses.
+ * Like the operators' above it is zero before its first use and its counters
+ * are left at zero; it serves every batch of up to n_seqs sequences with these
+ * heads. */
 UOCR_API size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads,
                                                         uint32_t head_dim);
 

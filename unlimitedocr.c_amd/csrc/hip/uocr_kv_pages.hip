@@ -174,15 +174,42 @@ __global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb) 
 
 constexpr u32 PA_TILE = 128;   /* tokens of a block's tile: 32 of each of its 4 wavefronts */
 constexpr u32 PA_BLOCKS = 512; /* 2 per CU: what the registers of a wavefront allow */
+constexpr u32 ALIGNED = 4;     /* most tiles of a block that has one set alone */
+constexpr u32 FUSED_ROWS = 512; /* most rows of partials that the last block of a set joins */
 
 struct PagedGrid {
     uocr_paged_args a;
     u32 group, chunks; /* query heads of a KV head; sets of up to 16 of them */
     u32 rows;          /* of a partial: min(group, 16) */
     float c;           /* scale * log2(e) */
+    u32 *count;        /* [n_seqs][sets]: partials that have arrived, 0 between launches */
+    bool fused;        /* the last block of a set joins it */
+    bool aligned;      /* few enough sets for a block each */
 };
 
 __device__ const uint4 g_zero_row[16] = {};
+
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+
+/* Cached rows are read once: non-temporal loads, 154 against 285 us at 876 MB
+ * of fp16 cache (5.7 TB/s) and 18.6 against 24.6 at 41 MB that the caches hold
+ * from call to call; Q8_0 pages, which need half the lines, 70 against 71. */
+__device__ __forceinline__ uint4 load_once(const uint8_t *p) {
+    const u32x4 v = __builtin_nontemporal_load((const u32x4 *)p);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+/* Partials go from block to block within a launch: stores and loads that pass
+ * the L2 of an XCD by (sc1), counted in by an atomic once they have arrived. */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t device_buffer(const void *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ void store_through(float *base, u32 at, f32x4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), device_buffer(base), at * 4u, 0, 16);
+}
+__device__ __forceinline__ f32x4 load_through(const float *base, u32 at) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(device_buffer(base), at * 4u, 0, 16));
+}
 
 /* Tokens of sequence s, and the tiles of each of its head sets. */
 __device__ __forceinline__ u32 seq_len(const uocr_paged_args &a, u32 s) {
@@ -192,52 +219,123 @@ __device__ __forceinline__ u32 len_tiles(u32 len) {
     return max((len + PA_TILE - 1u) / PA_TILE, 1u); /* an empty sequence has its zeros to write */
 }
 
-/* The block's share of all tiles.  Tiles are numbered by sequence, head set and
- * position; block b of G takes [N b / G, N (b + 1) / G), whatever sequences
- * these belong to, so no length of one sequence leaves CUs idle. */
-__device__ __forceinline__ u32 busy_blocks(uint64_t n, u32 g) {
-    return n < g ? (u32)n : g; /* none without a tile */
+/* Which block takes which tiles.  Tiles are numbered by sequence, head set and
+ * position.  Where a block has many, block b takes [N b / B, N (b + 1) / B) of
+ * all N, whatever sequences these belong to: no length of one sequence leaves
+ * CUs idle.  Where it has few (q of them, at most ALIGNED + 1), a set's tiles
+ * are padded to a multiple of q, if the blocks still run at once, and none
+ * begins a second set, whose loads would wait for the first one's end (16 sequences of about 1,044 tokens, Q8_0,
+ * 10 heads: 19.1 us, else 19.9; of 500 tokens fp16 17.3, else 19.8; with up to 9 tiles a
+ * block 2,000 tokens took 38.7 us against 35.6). */
+struct Split {
+    uint64_t total;
+    u32 q, blocks; /* q 0: any tiles */
+};
+__device__ __forceinline__ u32 padded(const Split &p, u32 nt) {
+    return p.q == 0u ? nt : (nt + p.q - 1u) / p.q * p.q;
 }
-__device__ __forceinline__ uint64_t share(uint64_t n, u32 b, u32 g) {
-    return n * b / g;
+__device__ __forceinline__ uint64_t share(const Split &p, u32 b) {
+    return p.q == 0u ? p.total * b / p.blocks : (uint64_t)b * p.q;
 }
-__device__ __forceinline__ u32 block_of(uint64_t n, uint64_t tile, u32 g) {
-    return (u32)(((tile + 1u) * g - 1u) / n);
+__device__ __forceinline__ u32 block_of(const Split &p, uint64_t tile) {
+    return (u32)(p.q == 0u ? ((tile + 1u) * p.blocks - 1u) / p.total : tile / p.q);
+}
+/* Place of a block's partial of the set that begins at tile T0: only without
+ * padding can it have two, of its first set and of its last. */
+__device__ __forceinline__ u32 place(const Split &p, u32 b, uint64_t T0) {
+    return p.q != 0u ? b : 2u * b + (share(p, b) >= T0 ? 0u : 1u);
 }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
     return ((uint64_t)(u32)__shfl_up((int)(v >> 32), d) << 32) | (u32)__shfl_up((int)v, d);
 }
 
-/* Prefix sums over the sequences' tiles, by the 256 threads of a block: every
- * thread takes a run of sequences.  Returns the tiles before the thread's run
- * and, in total, all tiles. */
-__device__ __forceinline__ uint64_t tiles_before(const PagedGrid &g, u32 run, uint64_t *total, uint64_t *red) {
-    const u32 t = threadIdx.x, sets = g.a.kv.heads * g.chunks;
-    uint64_t own = 0;
-    for (u32 s = t * run; s < min(t * run + run, g.a.kv.n_seqs); ++s) own += (uint64_t)len_tiles(seq_len(g.a, s)) * sets;
-    uint64_t sum = own;
+/* The split, and the tiles (padded) before the lane's run of sequences, by each
+ * wavefront for itself. */
+__device__ __forceinline__ uint64_t make_split(const PagedGrid &g, u32 run, Split &p) {
+    const u32 lane = threadIdx.x & 63u, sets = g.a.kv.heads * g.chunks, s0 = lane * run, s1 = min(s0 + run, g.a.kv.n_seqs);
+    const u32 nt0 = s0 < s1 ? len_tiles(seq_len(g.a, s0)) : 0u; /* mostly the only one */
+    auto sum = [&](uint64_t &own) {
+        own = padded(p, nt0);
+        for (u32 s = s0 + 1u; s < s1; ++s) own += padded(p, len_tiles(seq_len(g.a, s)));
+        own *= sets;
+        uint64_t all = own;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t v = shfl_up64(sum, d);
-        if ((int)(t & 63u) >= d) sum += v;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t v = shfl_up64(all, d);
+            if ((int)lane >= d) all += v;
+        }
+        p.total = (uint64_t)(u32)__builtin_amdgcn_readlane((int)all, 63) | ((uint64_t)(u32)__builtin_amdgcn_readlane((int)(all >> 32), 63) << 32);
+        return all - own;
+    };
+    p.q = 0u;
+    uint64_t own, before = sum(own);
+    const uint64_t n = p.total, q = (n + PA_BLOCKS - 1u) / PA_BLOCKS;
+    if (g.aligned && q <= ALIGNED) {
+        for (p.q = (u32)q; p.q <= (u32)q + 1u; ++p.q) {
+            const uint64_t with = p.q == 1u ? before : sum(own);
+            if (p.total > (uint64_t)PA_BLOCKS * p.q) continue; /* a second round of blocks would cost more */
+            p.blocks = (u32)(p.total / p.q);
+            return with;
+        }
+        p.q = 0u;
+        p.total = n;
     }
-    if ((t & 63u) == 63u) red[t >> 6] = sum;
-    __syncthreads();
-    uint64_t before = sum - own, all = 0;
-#pragma unroll
-    for (u32 w = 0; w < 4; ++w) {
-        if (w < (t >> 6)) before += red[w];
-        all += red[w];
-    }
-    *total = all;
+    p.blocks = (u32)min(n, (uint64_t)PA_BLOCKS); /* none without a tile */
     return before;
+}
+
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, u32 lane) {
+    return (uint64_t)(u32)__builtin_amdgcn_readlane((int)v, (int)lane) | ((uint64_t)(u32)__builtin_amdgcn_readlane((int)(v >> 32), (int)lane) << 32);
 }
 
 /* What a state with maximum m counts for beside one with maximum M >= m.  Only
  * scores that are all NaN leave weight without a maximum: their NaN goes on. */
 __device__ __forceinline__ float state_factor(float m, float M, float c) {
     return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * c);
+}
+
+/* Joins the partials of n heads (rows row0 .. of their set) that blocks b0 .. b1
+ * had tiles of (the set's tiles begin at T0): out = sum_b o_b 2^((m_b - M) c) /
+ * sum_b l_b 2^((m_b - M) c).  A group of n D / 4 threads reads every par-th
+ * partial, with the running maximum; the groups are joined through LDS. */
+template <int D>
+__device__ __forceinline__ void join_heads(const PagedGrid &g, const Split &sp, uint64_t T0, u32 b0, u32 b1, u32 row0, u32 n, uint16_t *out, uint8_t *sm) {
+    constexpr u32 LN = D / 4;
+    f32x4 *acc = (f32x4 *)sm;               /* [256] */
+    float2 *state = (float2 *)(acc + 256);  /* [256] */
+    const u32 t = threadIdx.x, lanes = n * LN, par = 256u / lanes, p = t / lanes, h = t % lanes / LN, ln = t % LN;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float m2, float l2, f32x4 v2) {
+        if (l2 == 0.0f) return; /* no weight there */
+        const float M = fmaxf(m, m2), f = l == 0.0f ? 0.0f : state_factor(m, M, g.c), f2 = state_factor(m2, M, g.c);
+        m = M;
+        l = fmaf(l2, f2, l * f);
+#pragma unroll
+        for (u32 e = 0; e < 4; ++e) v[e] = fmaf(v2[e], f2, v[e] * f);
+    };
+    if (p < par) {
+#pragma unroll 4
+        for (u32 b = b0 + p; b <= b1; b += par) {
+            const u32 at = (place(sp, b, T0) * g.rows + row0 + h) * (D + 4);
+            const f32x4 ml = load_through(g.a.part, at + D), o = load_through(g.a.part, at + 4u * ln);
+            add(ml.x, ml.y, o);
+        }
+    }
+    acc[t] = v;
+    state[t] = make_float2(m, l);
+    __syncthreads();
+    if (t < lanes) {
+        for (u32 x = 1; x < par; ++x) {
+            const float2 s2 = state[x * lanes + t];
+            add(s2.x, s2.y, acc[x * lanes + t]);
+        }
+        const float li = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (u32 e = 0; e < 4; ++e) out[h * D + 4u * ln + e] = __builtin_bit_cast(uint16_t, (h16)(v[e] * li));
+    }
+    __syncthreads();
 }
 
 /* One pass over the cache with the running maximum and sum of the softmax.
@@ -260,7 +358,8 @@ __device__ __forceinline__ float state_factor(float m, float M, float c) {
  *
  * The wavefronts' states are merged in LDS; a head set that one block covers is
  * written at once, else its fp32 state goes to the block's partials (at most
- * two: its first and its last set) for k_paged_join. */
+ * two: its first and its last set), which the last block to come, or
+ * k_paged_join, joins. */
 template <int D, bool Q8>
 __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
     constexpr u32 ROW = D * (Q8 ? 1 : 2);      /* bytes of a cached row */
@@ -271,45 +370,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
     constexpr u32 WLDS = 16 * ORS * 4 > 64 * D ? 16 * ORS * 4 : 64 * D; /* V tile, later the state */
     __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * WLDS];
     __shared__ float sml[4][2][16];
-    __shared__ uint64_t red[4];
-    __shared__ u32 start_s;
-    __shared__ uint64_t start_n;
+    __shared__ u32 arrived;
     const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 15u, gr = lane >> 4;
     const uocr_kv &kv = g.a.kv;
     const u32 sets = kv.heads * g.chunks;
 
-    uint64_t total;
-    const u32 run = (kv.n_seqs + 255u) / 256u;
-    const uint64_t before = tiles_before(g, run, &total, red);
-    const u32 blocks = busy_blocks(total, gridDim.x);
-    if (blockIdx.x >= blocks) return;
-    const uint64_t lo = share(total, blockIdx.x, blocks), hi = share(total, blockIdx.x + 1u, blocks);
-    {
-        /* the thread whose run holds tile lo finds its sequence */
-        uint64_t n = before;
-        const u32 s1 = min(t * run + run, kv.n_seqs);
-        for (u32 s = t * run; s < s1; ++s) {
-            const uint64_t next = n + (uint64_t)len_tiles(seq_len(g.a, s)) * sets;
-            if (n <= lo && lo < next) {
-                start_s = s;
-                start_n = n;
-            }
-            n = next;
-        }
-    }
-    __syncthreads();
-    u32 s = start_s;
-    uint64_t base = start_n, at = lo;
+    Split sp;
+    const u32 run = (kv.n_seqs + 63u) / 64u;
+    const uint64_t before = make_split(g, run, sp);
+    if (blockIdx.x >= sp.blocks) return;
+    const uint64_t lo = share(sp, blockIdx.x), hi = share(sp, blockIdx.x + 1u);
+    /* the last lane whose run begins at or before tile lo has its sequence (each has a tile) */
+    const u32 at_lane = 63u - (u32)__builtin_clzll(__ballot(before <= lo && lane * run < kv.n_seqs));
+    u32 s = at_lane * run;
+    uint64_t base = from_lane(before, at_lane), at = lo;
     uint8_t *vt = sm + wave * WLDS;
-    bool first = true;
     while (at < hi) {
-        const u32 len = seq_len(g.a, s), nt = len_tiles(len);
-        if (at >= base + (uint64_t)nt * sets) {
-            base += (uint64_t)nt * sets;
+        const u32 len = seq_len(g.a, s), nt = len_tiles(len), ntp = padded(sp, nt);
+        if (at >= base + (uint64_t)ntp * sets) {
+            base += (uint64_t)ntp * sets;
             ++s;
             continue;
         }
-        const u32 set = (u32)((at - base) / nt), ta = (u32)((at - base) % nt);
+        const u32 set = (u32)((at - base) / ntp), ta = (u32)((at - base) % ntp);
         const u32 tb = (u32)min((uint64_t)nt, (uint64_t)ta + (hi - at)); /* the block's tiles of this set: [ta, tb) */
         const u32 kvh = set / g.chunks, h0 = kvh * g.group + 16u * (set % g.chunks);
         const u32 nh = min(16u, kvh * g.group + g.group - h0); /* query heads of the set */
@@ -355,10 +438,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
             for (u32 n = 0; n < 2; ++n) {
                 const uint8_t *r = row(k, 16u * n + col) + 16u * gr;
 #pragma unroll
-                for (u32 x2 = 0; x2 < NK; ++x2) kr[n * NK + x2] = *(const uint4 *)(r + 64u * x2);
+                for (u32 x2 = 0; x2 < NK; ++x2) kr[n * NK + x2] = load_once(r + 64u * x2);
             }
 #pragma unroll
-            for (u32 y = 0; y < NV; ++y) vr[y] = *(const uint4 *)(row(v, (64u / VL) * y + lane / VL) + 16u * (lane % VL));
+            for (u32 y = 0; y < NV; ++y) vr[y] = load_once(row(v, (64u / VL) * y + lane / VL) + 16u * (lane % VL));
             if constexpr (Q8) {
                 ksc = vsc = 0u;
                 if (p >= 0) {
@@ -489,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
         }
         __syncthreads();
         const bool whole = ta == 0u && tb == nt;
-        const u32 slot = 2u * blockIdx.x + (first ? 0u : 1u);
+        const u32 slot = place(sp, blockIdx.x, base + (uint64_t)set * ntp);
         for (u32 i = t; i < nh * (D / 4); i += 256u) {
             const u32 h = i / (D / 4), d = 4u * (i % (D / 4));
             const float M = fmaxf(fmaxf(sml[0][0][h], sml[1][0][h]), fmaxf(sml[2][0][h], sml[3][0][h]));
@@ -511,83 +594,51 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
 #pragma unroll
                 for (u32 e = 0; e < 4; ++e) dst[e] = __builtin_bit_cast(uint16_t, (h16)(v[e] * li));
             } else {
-                float *part = g.a.part + (uint64_t)slot * g.rows * (D + 4);
-                *(f32x4 *)(part + h * (D + 4) + d) = v;
-                if (d == 0u) *(float2 *)(part + h * (D + 4) + D) = make_float2(M, L);
+                const u32 to = (slot * g.rows + h) * (D + 4);
+                store_through(g.a.part, to + d, v);
+                if (d == 0u) store_through(g.a.part, to + D, f32x4{M, L, 0.0f, 0.0f});
             }
         }
+        if (!whole && g.fused) {
+            /* the block that comes last joins the set's partials */
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const uint64_t T0 = base + (uint64_t)set * ntp;
+            const u32 b0 = block_of(sp, T0), b1 = block_of(sp, T0 + ntp - 1u);
+            if (t == 0u) {
+                u32 *count = g.count + (uint64_t)s * sets + set;
+                arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (arrived == b1 - b0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (arrived == b1 - b0) {
+                asm volatile("" ::: "memory");
+                constexpr u32 MOST = 256 / (D / 4);
+                for (u32 h = 0; h < nh; h += MOST)
+                    join_heads<D>(g, sp, T0, b0, b1, h, min(nh - h, MOST), g.a.out + (uint64_t)s * g.a.os + (h0 + h) * D, sm);
+            }
+        }
+        if (sp.q != 0u) break;
         __syncthreads();
         at += tb - ta;
-        first = false;
     }
 }
 
-/* Joins the partials of a head that several blocks had tiles of:
- * out = sum_b o_b 2^((m_b - M) c) / sum_b l_b 2^((m_b - M) c).  A block for
- * each sequence and head; 256 / (D / 4) partials are read at a time. */
+/* The join as a launch of its own, a block for each sequence and head. */
 template <int D>
-__global__ __launch_bounds__(256) void k_paged_join(PagedGrid g, u32 grid) {
-    constexpr u32 LN = D / 4, PAR = 256 / LN;
-    __shared__ uint64_t red[4], before_s;
-    __shared__ float wm[4];
-    __shared__ f32x4 acc[PAR][LN];
-    __shared__ float lsum[PAR];
-    const u32 t = threadIdx.x, s = blockIdx.x / g.a.hq, h = blockIdx.x % g.a.hq;
+__global__ __launch_bounds__(256) void k_paged_join(PagedGrid g) {
+    __shared__ __attribute__((aligned(16))) uint8_t sm[256 * 24];
+    const u32 s = blockIdx.x / g.a.hq, h = blockIdx.x % g.a.hq;
     const uocr_kv &kv = g.a.kv;
     const u32 kvh = h / g.group, set = kvh * g.chunks + h % g.group / 16u, row = h % g.group % 16u, sets = kv.heads * g.chunks;
-    const u32 nt = len_tiles(seq_len(g.a, s));
-    uint64_t total;
-    const u32 run = (kv.n_seqs + 255u) / 256u;
-    uint64_t before = tiles_before(g, run, &total, red);
-    if (s / run == t) {
-        for (u32 i = t * run; i < s; ++i) before += (uint64_t)len_tiles(seq_len(g.a, i)) * sets;
-        before_s = before;
-    }
-    __syncthreads();
-    const u32 blocks = busy_blocks(total, grid);
-    const uint64_t T0 = before_s + (uint64_t)set * nt;
-    const u32 b0 = block_of(total, T0, blocks), b1 = block_of(total, T0 + nt - 1u, blocks);
-    if (b0 == b1) return; /* one block had all of it */
-    auto part = [&](u32 b) { /* the set is the block's first unless the block began before it */
-        return g.a.part + ((uint64_t)(2u * b + (share(total, b, blocks) >= T0 ? 0u : 1u)) * g.rows + row) * (D + 4);
-    };
-    float M = -INFINITY;
-    for (u32 b = b0 + t; b <= b1; b += 256u) M = fmaxf(M, part(b)[D]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    if ((t & 63u) == 0u) wm[t >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    const u32 ln = t % LN, p = t / LN;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float L = 0.0f;
-    for (u32 b = b0 + p; b <= b1; b += PAR) {
-        const float *x = part(b);
-        const float2 ml = *(const float2 *)(x + D);
-        const f32x4 o = *(const f32x4 *)(x + 4u * ln);
-        if (ml.y == 0.0f) continue; /* no weight there */
-        const float f = state_factor(ml.x, M, g.c);
-        L = fmaf(ml.y, f, L);
-#pragma unroll
-        for (u32 e = 0; e < 4; ++e) v[e] = fmaf(o[e], f, v[e]);
-    }
-    acc[p][ln] = v;
-    if (ln == 0u) lsum[p] = L;
-    __syncthreads();
-    if (t < LN) {
-        L = lsum[0];
-#pragma unroll
-        for (u32 x = 1; x < PAR; ++x) {
-            L += lsum[x];
-            const f32x4 o = acc[x][t];
-#pragma unroll
-            for (u32 e = 0; e < 4; ++e) v[e] += o[e];
-        }
-        const float li = L == 0.0f ? 0.0f : 1.0f / L;
-        uint16_t *dst = g.a.out + (uint64_t)s * g.a.os + h * D + 4u * t;
-#pragma unroll
-        for (u32 e = 0; e < 4; ++e) dst[e] = __builtin_bit_cast(uint16_t, (h16)(v[e] * li));
-    }
+    Split sp;
+    const u32 run = (kv.n_seqs + 63u) / 64u;
+    const uint64_t before = make_split(g, run, sp);
+    const u32 ntp = padded(sp, len_tiles(seq_len(g.a, s)));
+    uint64_t T0 = from_lane(before, s / run) + (uint64_t)set * ntp;
+    for (u32 i = s / run * run; i < s; ++i) T0 += (uint64_t)padded(sp, len_tiles(seq_len(g.a, i))) * sets;
+    const u32 b0 = block_of(sp, T0), b1 = block_of(sp, T0 + ntp - 1u);
+    if (b0 != b1) join_heads<D>(g, sp, T0, b0, b1, row, 1u, g.a.out + (uint64_t)s * g.a.os + h * D, sm);
 }
 
 }  // namespace
@@ -622,9 +673,15 @@ hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
     return hipGetLastError();
 }
 
-size_t uocr_paged_attention_ws_bytes(uint32_t heads, uint32_t kv_heads, uint32_t dim) {
-    const u32 group = heads / kv_heads, rows = group < 16u ? group : 16u;
+namespace {
+size_t partial_bytes(u32 rows, u32 dim) {
     return (size_t)2u * PA_BLOCKS * rows * (dim + 4u) * sizeof(float);
+}
+}  // namespace
+
+size_t uocr_paged_attention_ws_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
+    const u32 group = heads / kv_heads, chunks = (group + 15u) / 16u;
+    return partial_bytes(group < 16u ? group : 16u, dim) + (size_t)n_seqs * kv_heads * chunks * sizeof(u32);
 }
 
 hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a) {
@@ -634,8 +691,13 @@ hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a)
     g.chunks = (g.group + 15u) / 16u;
     g.rows = g.group < 16u ? g.group : 16u;
     g.c = a->scale * 1.4426950408889634f;
+    g.count = (u32 *)((uint8_t *)a->part + partial_bytes(g.rows, a->kv.dim));
+    /* A set has at most PA_BLOCKS / sets + 2 partials (all sets of a sequence have as many tiles).  One block reads them
+     * one after another, the launch of its own with a block for each head: that pays where they are many. */
+    g.fused = (PA_BLOCKS / (a->kv.heads * g.chunks) + 2u) * g.rows <= FUSED_ROWS;
     const uint64_t most = ((uint64_t)(a->kv.table_stride << a->kv.shift) + PA_TILE - 1u) / PA_TILE; /* tiles of a set */
     const uint64_t tiles = most * a->kv.n_seqs * a->kv.heads * g.chunks;
+    g.aligned = (uint64_t)a->kv.n_seqs * a->kv.heads * g.chunks <= PA_BLOCKS;
     const u32 blocks = tiles < PA_BLOCKS ? (u32)tiles : PA_BLOCKS;
     if (a->kv.dim == 128u) {
         if (a->kv.q8) hipLaunchKernelGGL((k_paged_attention<128, true>), dim3(blocks), dim3(256), 0, st, g);
@@ -645,9 +707,9 @@ hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a)
         else hipLaunchKernelGGL((k_paged_attention<64, false>), dim3(blocks), dim3(256), 0, st, g);
     }
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || most == 1u) return e; /* one tile a set: nothing to join */
+    if (e != hipSuccess || g.fused || most == 1u) return e; /* one tile a set: nothing to join */
     const dim3 grid(a->kv.n_seqs * a->hq);
-    if (a->kv.dim == 128u) hipLaunchKernelGGL((k_paged_join<128>), grid, dim3(256), 0, st, g, blocks);
-    else hipLaunchKernelGGL((k_paged_join<64>), grid, dim3(256), 0, st, g, blocks);
+    if (a->kv.dim == 128u) hipLaunchKernelGGL((k_paged_join<128>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_paged_join<64>), grid, dim3(256), 0, st, g);
     return hipGetLastError();
 }
