@@ -12,23 +12,57 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+
+/* Cached rows are read once: non-temporal loads, 154 against 285 us at 876 MB
+ * of fp16 cache (5.7 TB/s) and 18.6 against 24.6 at 41 MB that the caches hold
+ * from call to call; Q8_0 pages, which need half the lines, 70 against 71. */
+__device__ __forceinline__ uint4 load_once(const uint8_t *p) {
+    const u32x4 v = __builtin_nontemporal_load((const u32x4 *)p);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 constexpr u32 APPEND_TOKENS = 8; /* most tokens of a block */
+constexpr u32 APPEND_ITEMS = 1;  /* rows' pieces of a thread that are loaded at a time */
 
 /* ---- append ----------------------------------------------------------------- */
 
 /* y1 = x1 cos - x2 sin, y2 = x1 sin + x2 cos on the pairs (i, i + D/2) of a
  * head.  A row is D/16 lanes, each 8 values of the low half and their partners.
- * Bound by HBM: every row is read and written once.  The angle is formed in
- * turns in fp64 and reduced to half a turn before the fp32 sine and cosine
- * (position 10^6 in fp32 would be off by 0.06 radians); a block computes them
- * once per token, in LDS, for all its heads. */
+ * Bound by HBM: every row is read and written once.  A thread's rows are loaded
+ * before the block finds its tokens' pages and angles, so that the two chains
+ * of loads run side by side.  The angle is formed in turns in fp64 and reduced
+ * to half a turn before the fp32 sine and cosine (position 10^6 in fp32 would
+ * be off by 0.06 radians); a block computes them once per token, in LDS, for
+ * all its heads. */
+/* 8 blocks of a CU: with the registers that the compiler takes by itself (3 blocks) 16,000 fp16 tokens of 32 + 8 heads
+ * take 128 us, so 82 (5.2 TB/s, a large copy's rate). */
 template <int D, bool Q8>
-__global__ __launch_bounds__(256) void k_kv_append(uocr_append_args a, u32 tpb) {
-    constexpr u32 LPR = D / 16;
+__global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tpb) {
+    constexpr u32 LPR = D / 16, U = APPEND_ITEMS;
     __shared__ float2 cs[APPEND_TOKENS][D / 2];
     __shared__ int page_of[APPEND_TOKENS], pos_of[APPEND_TOKENS];
     const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
+    const u32 kvh = a.kv.heads, rows = a.heads + 2u * kvh, items = nt * rows * LPR;
+    auto source = [&](u32 tok, u32 r) {
+        const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
+        const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
+        return (is_q ? a.q + (t0 + tok) * a.qs : is_v ? a.v + (t0 + tok) * a.vs : a.k + (t0 + tok) * a.ks) + h * D;
+    };
+    uint4 raw[2 * U];
+    auto load = [&](u32 first) {
+#pragma unroll
+        for (u32 u = 0; u < U; ++u) {
+            const u32 i = first + 256u * u;
+            if (i >= items) continue;
+            const uint16_t *src = source(i / LPR / rows, i / LPR % rows) + 8u * (i % LPR);
+            raw[2 * u] = load_any(src);
+            raw[2 * u + 1] = load_any(src + D / 2);
+        }
+    };
+    load(t);
     if (a.rotate) {
+#pragma unroll 1
         for (u32 i = t; i < nt * (D / 2); i += 256u) {
             const u32 tok = i / (D / 2), d = i % (D / 2);
             const double turns = (double)a.pos[t0 + tok] * (exp2((double)d * (-2.0 / D) * a.log2_theta) * 0.15915494309189535);
@@ -44,77 +78,89 @@ __global__ __launch_bounds__(256) void k_kv_append(uocr_append_args a, u32 tpb) 
         page_of[t] = in ? kv_page(a.kv, seq, (u32)pos) : -1;
     }
     __syncthreads();
-    const u32 kvh = a.kv.heads, rows = a.heads + 2u * kvh, items = nt * rows * LPR;
-    for (u32 i = t; i < items; i += 256u) {
-        const u32 lane = i % LPR, tok = i / LPR / rows, r = i / LPR % rows;
-        const int pos = pos_of[tok];
-        if (pos < 0) continue; /* a padding row: the whole row's lanes leave together */
-        const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
-        const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
-        const uint16_t *src = (is_q ? a.q + (t0 + tok) * a.qs : is_v ? a.v + (t0 + tok) * a.vs : a.k + (t0 + tok) * a.ks) + h * D + 8u * lane;
-        U4H8 lo, hi;
-        lo.u = load_any(src);
-        hi.u = load_any(src + D / 2);
-        float y[16];
+#pragma unroll 1
+    for (u32 i0 = t; i0 < items; i0 += 256u * U) {
+        if (i0 != t) load(i0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x1 = (float)lo.h[e], x2 = (float)hi.h[e];
-            if (a.rotate && !is_v) {
-                const float2 w = cs[tok][8u * lane + e];
-                y[e] = fmaf(x1, w.x, -(x2 * w.y));
-                y[8 + e] = fmaf(x1, w.y, x2 * w.x);
+        for (u32 u = 0; u < U; ++u) {
+            const u32 i = i0 + 256u * u;
+            if (i >= items) continue;
+            const u32 lane = i % LPR, tok = i / LPR / rows, r = i / LPR % rows;
+            const int pos = pos_of[tok];
+            if (pos < 0) continue; /* a padding row: the whole row's lanes leave together */
+            const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
+            const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
+            U4H8 lo, hi;
+            lo.u = raw[2 * u];
+            hi.u = raw[2 * u + 1];
+            float y[16];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x1 = (float)lo.h[e], x2 = (float)hi.h[e];
+                if (a.rotate && !is_v) {
+                    const float2 w = cs[tok][8u * lane + e];
+                    y[e] = fmaf(x1, w.x, -(x2 * w.y));
+                    y[8 + e] = fmaf(x1, w.y, x2 * w.x);
+                } else {
+                    y[e] = x1;
+                    y[8 + e] = x2;
+                }
+                lo.h[e] = (h16)y[e];
+                hi.h[e] = (h16)y[8 + e];
+            }
+            uint16_t *rows_out = is_q ? a.q_out + (t0 + tok) * a.qos : is_v || a.k_out == nullptr ? nullptr : a.k_out + (t0 + tok) * a.kos;
+            if (rows_out != nullptr) {
+                store_any(rows_out + h * D + 8u * lane, lo.u);
+                store_any(rows_out + h * D + 8u * lane + D / 2, hi.u);
+            }
+            if (is_q || page_of[tok] < 0) continue;
+            const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u)); /* row of the page */
+            const uint64_t at = (uint64_t)page_of[tok] * a.kv.page_stride + (uint64_t)slot * D + 8u * lane;
+            if constexpr (!Q8) {
+                uint16_t *dst = (uint16_t *)(is_v ? a.kv.v : a.kv.k) + at;
+                *(uint4 *)dst = lo.u;
+                *(uint4 *)(dst + D / 2) = hi.u;
             } else {
-                y[e] = x1;
-                y[8 + e] = x2;
-            }
-            lo.h[e] = (h16)y[e];
-            hi.h[e] = (h16)y[8 + e];
-        }
-        uint16_t *rows_out = is_q ? a.q_out + (t0 + tok) * a.qos : is_v || a.k_out == nullptr ? nullptr : a.k_out + (t0 + tok) * a.kos;
-        if (rows_out != nullptr) {
-            store_any(rows_out + h * D + 8u * lane, lo.u);
-            store_any(rows_out + h * D + 8u * lane + D / 2, hi.u);
-        }
-        if (is_q || page_of[tok] < 0) continue;
-        const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u)); /* row of the page */
-        const uint64_t at = (uint64_t)page_of[tok] * a.kv.page_stride + (uint64_t)slot * D + 8u * lane;
-        if constexpr (!Q8) {
-            uint16_t *dst = (uint16_t *)(is_v ? a.kv.v : a.kv.k) + at;
-            *(uint4 *)dst = lo.u;
-            *(uint4 *)(dst + D / 2) = hi.u;
-        } else {
-            /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
-             * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8) */
-            float m0 = 0.0f, m1 = 0.0f;
+                /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
+                 * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8) */
+                float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                m0 = fabsf(y[e]) < INFINITY ? fmaxf(m0, fabsf(y[e])) : INFINITY;
-                m1 = fabsf(y[8 + e]) < INFINITY ? fmaxf(m1, fabsf(y[8 + e])) : INFINITY;
-            }
-            if (D == 64) m0 = m1 = fmaxf(m0, m1); /* both halves are one group */
+                for (int e = 0; e < 8; ++e) {
+                    m0 = fabsf(y[e]) < INFINITY ? fmaxf(m0, fabsf(y[e])) : INFINITY;
+                    m1 = fabsf(y[8 + e]) < INFINITY ? fmaxf(m1, fabsf(y[8 + e])) : INFINITY;
+                }
+                if (D == 64) m0 = m1 = fmaxf(m0, m1); /* both halves are one group */
 #pragma unroll
-            for (u32 o = 1; o < LPR; o <<= 1) {
-                m0 = fmaxf(m0, __shfl_xor(m0, o));
-                m1 = fmaxf(m1, __shfl_xor(m1, o));
-            }
-            union {
-                int8_t b[8];
-                uint2 u;
-            } q0, q1;
-            const float s0 = m0 == 0.0f ? 1.0f : m0 / 127.0f, s1 = m1 == 0.0f ? 1.0f : m1 / 127.0f;
+                for (u32 o = 1; o < LPR; o <<= 1) {
+                    m0 = fmaxf(m0, __shfl_xor(m0, o));
+                    m1 = fmaxf(m1, __shfl_xor(m1, o));
+                }
+                union {
+                    int8_t b[8];
+                    uint2 u;
+                } q0, q1;
+                const float s0 = m0 == 0.0f ? 1.0f : m0 / 127.0f, s1 = m1 == 0.0f ? 1.0f : m1 / 127.0f;
+                /* y / s rounded as a division is: the product with the rounded reciprocal, corrected by its residual
+                 * (Markstein's method; a quarter of a division's instructions, 28.9 against 30.9 us with the gather) */
+                const float i0 = 1.0f / s0, i1 = 1.0f / s1;
+                auto quotient = [](float v, float sc, float inv) {
+                    const float x = v * inv;
+                    return fmaf(fmaf(-x, sc, v), inv, x);
+                };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                /* a group that is not finite: 0 times its NaN scale */
-                q0.b[e] = m0 < INFINITY ? (int8_t)fminf(fmaxf(rintf(y[e] / s0), -127.0f), 127.0f) : (int8_t)0;
-                q1.b[e] = m1 < INFINITY ? (int8_t)fminf(fmaxf(rintf(y[8 + e] / s1), -127.0f), 127.0f) : (int8_t)0;
-            }
-            int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
-            *(uint2 *)dst = q0.u;
-            *(uint2 *)(dst + D / 2) = q1.u;
-            if (lane == 0u) {
-                uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
-                sc[0] = m0 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
-                if (D == 128) sc[1] = m1 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
+                for (int e = 0; e < 8; ++e) {
+                    /* a group that is not finite: 0 times its NaN scale */
+                    q0.b[e] = m0 < INFINITY ? (int8_t)fminf(fmaxf(rintf(quotient(y[e], s0, i0)), -127.0f), 127.0f) : (int8_t)0;
+                    q1.b[e] = m1 < INFINITY ? (int8_t)fminf(fmaxf(rintf(quotient(y[8 + e], s1, i1)), -127.0f), 127.0f) : (int8_t)0;
+                }
+                int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
+                *(uint2 *)dst = q0.u;
+                *(uint2 *)(dst + D / 2) = q1.u;
+                if (lane == 0u) {
+                    uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
+                    sc[0] = m0 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
+                    if (D == 128) sc[1] = m1 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
+                }
             }
         }
     }
@@ -125,7 +171,7 @@ __global__ __launch_bounds__(256) void k_kv_append(uocr_append_args a, u32 tpb) 
 /* A copy (Q8_0: fp16(q * scale)), bound by HBM: 8 or 16 values a lane, four
  * items of a thread in flight. */
 template <int D, bool Q8>
-__global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb) {
+__global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb, bool once) {
     constexpr u32 E = Q8 ? 16 : 8, LPR = D / E, U = 4;
     const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
     const u32 kvh = a.kv.heads, first = a.k_out == nullptr ? kvh : 0u, rows = (a.v_out == nullptr ? kvh : 2u * kvh) - first;
@@ -147,7 +193,8 @@ __global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb) 
             const bool is_v = r >= kvh;
             const u32 slot = ((is_v ? r - kvh : r) << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u));
             const uint64_t at = (uint64_t)page * a.kv.page_stride + (uint64_t)slot * D + E * lane;
-            w[u] = *(const uint4 *)((const uint8_t *)(is_v ? a.kv.v : a.kv.k) + (Q8 ? at : 2u * at));
+            const uint8_t *src = (const uint8_t *)(is_v ? a.kv.v : a.kv.k) + (Q8 ? at : 2u * at);
+            w[u] = once ? load_once(src) : *(const uint4 *)src;
             if (Q8) sc[u] = (is_v ? a.kv.vs : a.kv.ks)[(uint64_t)page * (a.kv.page_stride / 64u) + slot * (D / 64u) + lane / 4u];
         }
 #pragma unroll
@@ -188,16 +235,6 @@ struct PagedGrid {
 };
 
 __device__ const uint4 g_zero_row[16] = {};
-
-typedef u32 u32x4 __attribute__((ext_vector_type(4)));
-
-/* Cached rows are read once: non-temporal loads, 154 against 285 us at 876 MB
- * of fp16 cache (5.7 TB/s) and 18.6 against 24.6 at 41 MB that the caches hold
- * from call to call; Q8_0 pages, which need half the lines, 70 against 71. */
-__device__ __forceinline__ uint4 load_once(const uint8_t *p) {
-    const u32x4 v = __builtin_nontemporal_load((const u32x4 *)p);
-    return make_uint4(v.x, v.y, v.z, v.w);
-}
 
 /* Partials go from block to block within a launch: stores and loads that pass
  * the L2 of an XCD by (sc1), counted in by an atomic once they have arrived. */
@@ -662,13 +699,17 @@ hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
     const u32 sides = (a->k_out != nullptr ? 1u : 0u) + (a->v_out != nullptr ? 1u : 0u);
     const u32 lanes = sides * a->kv.heads * a->kv.dim / (a->kv.q8 ? 16u : 8u);
     const u32 tpb = lanes >= 1024u ? 1u : 1024u / lanes; /* 1,024 items: four of each thread */
+    /* Pages of many tokens are read past the caches (16,000 tokens of 8 heads of 128, eight caches in turn: fp16 29.8
+     * against 31.0 us, Q8_0 29.5 against 31.2), those of few may be there still (4,000 of 10: 9.9 against 12.9, 10.8
+     * against 12.8 with three in turn). */
+    const bool once = (uint64_t)a->tokens * lanes * 16u > (24u << 20);
     const dim3 grid((a->tokens + tpb - 1u) / tpb);
     if (a->kv.dim == 128u) {
-        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<128, true>), grid, dim3(256), 0, st, *a, tpb);
-        else hipLaunchKernelGGL((k_kv_gather<128, false>), grid, dim3(256), 0, st, *a, tpb);
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<128, true>), grid, dim3(256), 0, st, *a, tpb, once);
+        else hipLaunchKernelGGL((k_kv_gather<128, false>), grid, dim3(256), 0, st, *a, tpb, once);
     } else {
-        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<64, true>), grid, dim3(256), 0, st, *a, tpb);
-        else hipLaunchKernelGGL((k_kv_gather<64, false>), grid, dim3(256), 0, st, *a, tpb);
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<64, true>), grid, dim3(256), 0, st, *a, tpb, once);
+        else hipLaunchKernelGGL((k_kv_gather<64, false>), grid, dim3(256), 0, st, *a, tpb, once);
     }
     return hipGetLastError();
 }
