@@ -364,14 +364,24 @@ def test_packed_attention_lengths(gpu, dim, n):
     packed_case(gpu, rng, 1, 1, dim, [n, 1])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,nq,nk", [(24, [300, 1000], None), (12, [700, 1, 650], [700, 900, 651]), (40, [90] * 12, None), (16, [260, 129, 511, 400], None)],
+                         ids=["24x2", "12x3", "40x12", "16x4"])
+def test_packed_attention_tile_choices(gpu, dim, heads, nq, nk):
+    """Few long and many short prompts: every way of sharing out tiles; strided rows too."""
+    rng = np.random.default_rng(heads)
+    packed_case(gpu, rng, heads, 4, dim, nq, nk)
+    packed_case(gpu, rng, heads, 4, dim, nq, nk, gaps=(1, 3, 3, 1), shift=1)
+
+
 def test_packed_attention_many_short(gpu):
     rng = np.random.default_rng(3)
     packed_case(gpu, rng, 2, 1, 64, list(rng.integers(0, 6, 700)))
 
 
-@pytest.mark.parametrize("n", [150, 400])
+@pytest.mark.parametrize("heads,n", [(2, 150), (2, 400), (20, 700), (40, 400), (90, 400)])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_packed_attention_values_that_are_not_finite(gpu, dim, n):
+def test_packed_attention_values_that_are_not_finite(gpu, dim, heads, n):
     """Keys and values that a row does not see never reach it; those it sees go through."""
     rng = np.random.default_rng(4)
 
@@ -380,7 +390,7 @@ def test_packed_attention_values_that_are_not_finite(gpu, dim, n):
         v[100, 0, 9], k[120, 0, 3] = np.nan, np.nan
         v[n - 1, 0, :], k[n, 0, :], v[n, 0, :] = np.nan, np.nan, np.inf
 
-    packed_case(gpu, rng, 2, 1, dim, [n, 50], change=change)
+    packed_case(gpu, rng, heads, 1, dim, [n, 50], change=change)
 
 
 def test_packed_attention_bad_starts(gpu):
