@@ -40,7 +40,7 @@ def attend(q, k, v, seen, scale, v_rounded=False):
     Returns the result and its bound.  Scores: fp32 sums of dim exact products,
     dim 2^-24 sum |q k| each, and the exponent's argument rounds twice; so a
     weight is off by delta, at most twice that in the quotient.  Weights round
-    to fp16 (2^-11, or 2^-25 of the largest weight 1); their sum and the sum of
+    to fp16 (2^-11, or 2^-25 beside a largest one of 1 to 256); their sum and the sum of
     products round once per key in fp32.  Q8_0 values enter as fp16."""
     rows, dim = q.shape
     out, tol = np.zeros((rows, v.shape[1])), np.zeros((rows, v.shape[1]))

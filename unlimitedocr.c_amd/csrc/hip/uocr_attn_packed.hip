@@ -55,8 +55,10 @@ __device__ __forceinline__ u32 start_of(const int32_t *starts, u32 s, u32 tokens
     return (u32)min(max(starts[s], 0), (int)tokens);
 }
 
-/* Bound by the matrix and vector pipes (per 32 x 32 scores 512 cycles of MFMA,
- * about 450 of exponentials, maxima and conversions with head_dim 128).
+/* Bound by the power that the matrix unit may draw: 4 x 4,001 rows of 32 heads
+ * run at 894 TFLOP/s and 2.0 GHz, the library's fp16 product of 8,192 x 8,192
+ * x 8,192 at 1,134 and 1.84 GHz.  Multiplying the next tile's K beside this
+ * one's exponentials, or reading K operands further ahead, changed nothing.
  *
  * Block: WQ x 32 query rows of one sequence and head; its wavefronts are WG key
  * groups of WQ wavefronts, group g takes the key tiles g, g + WG, .. of the
@@ -126,8 +128,6 @@ __global__ __launch_bounds__(64 * WQ * WG, 2) void k_packed_attention(PackedGrid
     };
 
     U4H8 qreg[D / 16];
-#pragma unroll
-    for (u32 x = 0; x < D / 16; ++x) qreg[x].u = load_any(a.q + (uint64_t)(qa + qmax) * a.qs + h * D + 16u * x + 8u * hf);
     f32x16 o[D / 32];
     float m, l; /* m in units of the raw scores; l: this lane's half of the sum */
     auto attend = [&](auto special) {
@@ -141,6 +141,12 @@ __global__ __launch_bounds__(64 * WQ * WG, 2) void k_packed_attention(PackedGrid
 #pragma unroll
             for (u32 b = 0; b + 1u < NB; ++b) issue(min(b * WG + gi, nt - 1u), b);
         }
+#pragma unroll
+        for (u32 x = 0; x < D / 16; ++x) qreg[x].u = load_any(a.q + (uint64_t)(qa + qmax) * a.qs + h * D + 16u * x + 8u * hf);
+        /* The queries are waited for here.  Left to their first use, in the loop, the compiler's wait counts the tiles'
+         * loads, which it does not know of, and stops every pass until the next tile has come as well. */
+#pragma unroll
+        for (u32 x = 0; x < D / 16; ++x) asm volatile("" : "+v"(qreg[x].v));
         u32 buf = 0;
         for (u32 it = 0; it < iters; ++it) {
             /* tile it has landed for all wavefronts; its predecessor's buffer is free */
@@ -174,7 +180,9 @@ __global__ __launch_bounds__(64 * WQ * WG, 2) void k_packed_attention(PackedGrid
                 for (int i = 0; i < 16; ++i) tm = fmaxf(tm, sc[n][i]);
             }
             tm = fmaxf(tm, __shfl_xor(tm, 32));
-            if (__any(tm > m)) { /* only when some row's maximum grew */
+            /* The reference point follows a row's maximum at a distance of up to 2^8 (weights of up to 256 round to fp16
+             * as those up to 1 do): most tiles then rescale nothing, 470 -> 452 us for 9,900 rows of 32 heads. */
+            if (__any((tm - m) * g.c > 8.0f)) {
                 const float mn = fmaxf(m, tm), corr = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * g.c);
                 m = mn;
                 l *= corr;
@@ -341,6 +349,7 @@ hipError_t launch(hipStream_t st, const uocr_packed_args &a) {
 /* Measured (us; wavefronts along queries x along keys, keys per tile; head_dim
  * 128; x: tiles of 128 rows, all heads, and one more for each sequence):
  *   heads x sequences x rows     x     4 x 1, 64   2 x 4, 32   4 x 2, 64
+ *   10 x 1 x 64                  10         7.7         9.6         9.7
  *   10 x 1 x 932                 80        25.1        18.9        24.5
  *   10 x 1 x 2500               200        65.7        42.7        57.8
  *   32 x 1 x 700                192        20.4        21.0        20.8
@@ -355,7 +364,7 @@ hipError_t launch(hipStream_t st, const uocr_packed_args &a) {
 template <int D>
 hipError_t choose(hipStream_t st, const uocr_packed_args &a) {
     const uint64_t x = ((uint64_t)a.q_tokens / 128u + a.n_seqs) * a.heads, keys = a.k_tokens / a.n_seqs;
-    if (x <= 160u || (x <= 240u && keys >= 1000u)) return launch<D, 2, 4, 32, 2>(st, a);
+    if (keys >= 256u && (x <= 160u || (x <= 240u && keys >= 1000u))) return launch<D, 2, 4, 32, 2>(st, a);
     if (x <= 512u && keys >= 320u) return launch<D, 4, 2, 64, 2>(st, a);
     return launch<D, 4, 1, 64, 2>(st, a);
 }
