@@ -363,8 +363,8 @@ UOCR_API int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens, c
 
 /* Bytes of uocr_op_paged_attention's workspace, or 0 for sizes that it refuses.
  * Like the operators' above it is zero before its first use and its counters
- * are left at zero; it serves every batch of up to n_seqs sequences with these
- * heads. */
+ * are left at zero, so that calls of any sizes can take turns on one that is
+ * large enough for each. */
 UOCR_API size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads,
                                                         uint32_t head_dim);
 
@@ -373,8 +373,8 @@ UOCR_API size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_
  * out[s][h] = sum_j p_j v_j, p = softmax_j(scale q . k_j), KV head
  * h / (heads / kv_heads).  q and out fp16 [n_seqs][heads][head_dim], strides in
  * values from one sequence to the next (out may be q); scale 0: 1 /
- * sqrt(head_dim).  fp32 softmax and sums; probabilities and Q8_0 values enter
- * the products in fp16.  Tokens in absent pages are left out; where none is
+ * sqrt(head_dim).  fp32 softmax and sums; probabilities (Q8_0: times the
+ * values' scales) enter the products in fp16.  Tokens in absent pages are left out; where none is
  * left the row is zero.  Beside uocr_op_attention_decode. */
 UOCR_API int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_t *lengths, uint32_t heads, float scale,
                                      const void *q, uint64_t q_stride, void *workspace, void *out,

@@ -35,13 +35,15 @@ def stored(payload, scales):
     return payload.astype(np.float64) * np.repeat(scales.astype(np.float64), 64, -1)
 
 
-def attend(q, k, v, seen, scale, v_rounded=False):
+def attend(q, k, v, seen, scale, top=1.0):
     """One head: q [rows][dim], k, v [keys][dim] (fp64), seen [rows][keys].
     Returns the result and its bound.  Scores: fp32 sums of dim exact products,
     dim 2^-24 sum |q k| each, and the exponent's argument rounds twice; so a
     weight is off by delta, at most twice that in the quotient.  Weights round
     to fp16 (2^-11, or 2^-25 beside a largest one of 1 to 256); their sum and the sum of
-    products round once per key in fp32.  Q8_0 values enter as fp16."""
+    products round once per key in fp32.  Q8_0: it is a weight times its scale,
+    over up to twice the largest scale, that rounds; top is how much larger that
+    makes the least step beside a value (2 times largest over least scale)."""
     rows, dim = q.shape
     out, tol = np.zeros((rows, v.shape[1])), np.zeros((rows, v.shape[1]))
     for i in range(rows):
@@ -56,9 +58,7 @@ def attend(q, k, v, seen, scale, v_rounded=False):
         mass = w @ np.abs(v[j])
         delta = H32 * (scale * dim * (np.abs(k[j]) @ np.abs(q[i])).max() + 8 * np.abs(s).max() + 8)
         n = len(j)
-        tol[i] = mass * (H16 * (2 if v_rounded else 1) + 4 * delta + 4 * n * H32) + n * SUB16 * np.abs(v[j]).max(0) + H16 * np.abs(out[i]) + SUB16
-        if v_rounded:
-            tol[i] += SUB16
+        tol[i] = mass * (H16 + 4 * delta + 4 * n * H32) + n * top * SUB16 * np.abs(v[j]).max(0) + H16 * np.abs(out[i]) + SUB16
     return out, tol
 
 
@@ -158,7 +158,7 @@ class Pages:
         return other
 
 
-def paged(pages, lengths, q, scale):
+def paged(pages, lengths, q, scale, top=None):
     """[seqs][heads][dim] of one new token each, and the bound."""
     n, heads, dim = q.shape
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -169,7 +169,7 @@ def paged(pages, lengths, q, scale):
             k = np.array([pages.row(0, s, p, g) for p in rows]).reshape(len(rows), dim)
             v = np.array([pages.row(1, s, p, g) for p in rows]).reshape(len(rows), dim)
             per = heads // pages.kv_heads
-            o, t = attend(q[s, g * per:(g + 1) * per].astype(np.float64), k, v, np.ones((per, len(rows)), bool), scale, pages.qtype == 3)
+            o, t = attend(q[s, g * per:(g + 1) * per].astype(np.float64), k, v, np.ones((per, len(rows)), bool), scale, top or (8.0 if pages.qtype == 3 else 1.0))
             out[s, g * per:(g + 1) * per], tol[s, g * per:(g + 1) * per] = o, t
     return out, tol
 

@@ -191,7 +191,7 @@ def test_gather(gpu, qtype, kvh, dim, page):
 
 # ---- attention of one token ----------------------------------------------------------
 
-def paged_case(uocr, rng, qtype, heads, kvh, dim, page, lengths, scale=0.0, gap=0, absent=(), q_gap=0, shift=0, said=None, q=None, change=None):
+def paged_case(uocr, rng, qtype, heads, kvh, dim, page, lengths, scale=0.0, gap=0, absent=(), q_gap=0, shift=0, said=None, q=None, change=None, ws=None, top=None):
     c = Pages(rng, qtype, kvh, dim, page, lengths, gap=gap, absent=absent)
     c.fill(rng, lengths)
     if change:
@@ -205,7 +205,7 @@ def paged_case(uocr, rng, qtype, heads, kvh, dim, page, lengths, scale=0.0, gap=
     rows[:, :heads * dim] = q.reshape(n, -1)
     dq = dev(uocr, np.concatenate([np.zeros(shift, np.float16), rows.reshape(-1)]))
     out = dev(uocr, np.full(n * stride + shift, 9, np.float16))
-    ws = uocr.DeviceBuffer(uocr.paged_attention_workspace_bytes(n, heads, kvh, dim))
+    ws = ws or uocr.DeviceBuffer(uocr.paged_attention_workspace_bytes(n, heads, kvh, dim))
     dl = dev(uocr, np.array(said, np.int32))
     uocr.op_paged_attention(desc, dl, heads, scale, dq.ptr + 2 * shift, stride, ws, out.ptr + 2 * shift, stride)
     uocr.sync()
@@ -214,7 +214,7 @@ def paged_case(uocr, rng, qtype, heads, kvh, dim, page, lengths, scale=0.0, gap=
     got = got[shift:].reshape(n, stride)
     assert np.all(got[:, heads * dim:] == 9)
     got = got[:, :heads * dim].reshape(n, heads, dim)
-    ref, tol = paged(c, said, q, scale or dim ** -0.5)
+    ref, tol = paged(c, said, q, scale or dim ** -0.5, top)
     near(got, ref, tol, "paged")
     return got
 
@@ -278,6 +278,28 @@ def test_paged_attention_far_scores(gpu):
                 c.data[0][c.slot(1, p, h):][:128] = 25
 
     paged_case(gpu, rng, 1, 2, 1, 128, 32, [300, 300], scale=1.0, q=q, change=change)
+
+
+def test_paged_attention_one_workspace_for_all_sizes(gpu):
+    """Calls of different heads, dims and batches take turns on one workspace."""
+    rng = np.random.default_rng(14)
+    size = max(gpu.paged_attention_workspace_bytes(9, *h) for h in ((10, 10, 128), (32, 8, 64), (32, 1, 128)))
+    ws = gpu.DeviceBuffer(size)
+    for heads, kvh, dim, lengths in ((10, 10, 128, [932]), (32, 1, 128, [900, 2000]), (32, 8, 64, [300, 700, 1, 4000]), (4, 4, 128, [600] * 9)) * 2:
+        paged_case(gpu, rng, 1, heads, kvh, dim, 16, lengths, ws=ws)
+
+
+def test_paged_attention_q8_scales_far_apart(gpu):
+    """Scales that grow along the cache, by powers of two and more."""
+    rng = np.random.default_rng(15)
+
+    def change(c):
+        for p in range(400):
+            for h in range(2):
+                a = c.slot(0, p, h)
+                c.scales[1][a // 64:a // 64 + 2] = np.array([0.001 * 1.03 ** p, 2.0 ** (p // 40 - 12)], np.float16)
+
+    paged_case(gpu, rng, 3, 4, 2, 128, 16, [400], change=change, top=2.0 ** 18)
 
 
 def test_paged_attention_in_place_and_repeated(gpu):

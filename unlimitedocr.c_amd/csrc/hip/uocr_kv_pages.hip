@@ -229,7 +229,8 @@ struct PagedGrid {
     u32 group, chunks; /* query heads of a KV head; sets of up to 16 of them */
     u32 rows;          /* of a partial: min(group, 16) */
     float c;           /* scale * log2(e) */
-    u32 *count;        /* [n_seqs][sets]: partials that have arrived, 0 between launches */
+    u32 *count;        /* [PA_BLOCKS]: partials of the set that goes on behind a block, which is one at most, that have
+                        * arrived; 0 between launches, at the same place whatever the heads */
     bool fused;        /* the last block of a set joins it */
     bool aligned;      /* few enough sets for a block each */
 };
@@ -326,6 +327,11 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t v, u32 lane) {
     return (uint64_t)(u32)__builtin_amdgcn_readlane((int)v, (int)lane) | ((uint64_t)(u32)__builtin_amdgcn_readlane((int)(v >> 32), (int)lane) << 32);
 }
 
+/* The scale of group j, of two in a word. */
+__device__ __forceinline__ float scale_of(u32 pair, u32 j) {
+    return (float)__builtin_bit_cast(h16, (unsigned short)(j == 0u ? pair & 0xffffu : pair >> 16));
+}
+
 /* What a state with maximum m counts for beside one with maximum M >= m.  Only
  * scores that are all NaN leave weight without a maximum: their NaN goes on. */
 __device__ __forceinline__ float state_factor(float m, float M, float c) {
@@ -389,7 +395,9 @@ __device__ __forceinline__ void join_heads(const PagedGrid &g, const Split &sp, 
  *   O^T += V^T P^T: the probabilities stay where S^T left them, V goes through
  *   LDS, row-major, and is transposed by the LDS read.
  * Q8_0: K enters the MFMA as its integers (exact in fp16), a sum for each group
- * of 64 dims, the fp32 sums times the scales; V as fp16(q * scale).
+ * of 64 dims, the fp32 sums times the scales; V as its integers, too, and its
+ * scales, over a power of two above the largest so far, with the probabilities
+ * (one rounding to fp16 for both).
  * Tokens past the length or in absent pages are read from a row of zeros: what
  * stands there never enters a product.
  *
@@ -407,6 +415,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
     constexpr u32 WLDS = 16 * ORS * 4 > 64 * D ? 16 * ORS * 4 : 64 * D; /* V tile, later the state */
     __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * WLDS];
     __shared__ float sml[4][2][16];
+    __shared__ __attribute__((aligned(16))) u32 scales[4][2][32];
     __shared__ u32 arrived;
     const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 15u, gr = lane >> 4;
     const uocr_kv &kv = g.a.kv;
@@ -447,6 +456,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
 #pragma unroll
         for (u32 n = 0; n < D / 16; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
+        float unit = 0x1p30f; /* Q8_0: sums are in units of 1 / unit, a power of two */
 
         uint4 kr[2 * NK], vr[NV];
         u32 ksc = 0, vsc = 0; /* scales of token lane % 32 */
@@ -498,19 +508,36 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
         for (u32 x = ta; x < tb; ++x) {
             const u32 now = valid;
             float sc[8];
+            u32 sv[8]; /* Q8_0: the scales of V, where the scores are */
             if (now != 0u) {
                 /* V to LDS, rows swizzled by pairs of 16-byte pieces so that the transposing reads touch all banks */
                 __builtin_amdgcn_wave_barrier();
+                if (Q8 && lane < 32u) {
+                    scales[wave][0][lane] = ksc;
+                    scales[wave][1][lane] = vsc;
+                }
+                if constexpr (Q8) {
+                    const float top = fmaxf(fabsf(scale_of(vsc, 0)), fabsf(scale_of(vsc, 1)));
+                    if (__any(top * unit > 1.0f)) {
+                        float all = top;
+#pragma unroll
+                        for (int x2 = 32; x2 > 0; x2 >>= 1) all = fmaxf(all, __shfl_xor(all, x2));
+                        const float to = all < 65536.0f ? ldexpf(1.0f, -ilogbf(all) - 1) : 0x1p-16f, by = to / unit;
+                        unit = to;
+#pragma unroll
+                        for (u32 n = 0; n < D / 16; ++n)
+#pragma unroll
+                            for (u32 i = 0; i < 4; ++i) o[n][i] *= by;
+                    }
+                }
                 auto swz = [](u32 key, u32 pc) { return key * (2u * D) + 16u * (pc ^ (D == 128 ? (key & 7u) << 1 : ((key >> 1) & 3u) << 1)); };
 #pragma unroll
                 for (u32 y = 0; y < NV; ++y) {
                     const u32 key = (64u / VL) * y + lane / VL, pc = lane % VL;
                     if constexpr (Q8) {
-                        const u32 s2 = (u32)__shfl((int)vsc, (int)key);
-                        const u32 sv = pc >= 4u ? s2 >> 16 : s2 & 0xffffu;
                         U4H8 a, b;
-                        a.v = dequant_q8(vr[y].x, vr[y].y, sv);
-                        b.v = dequant_q8(vr[y].z, vr[y].w, sv);
+                        a.v = dequant_q8(vr[y].x, vr[y].y, 0x3c00u);
+                        b.v = dequant_q8(vr[y].z, vr[y].w, 0x3c00u);
                         *(uint4 *)(vt + swz(key, 2u * pc)) = a.u;
                         *(uint4 *)(vt + swz(key, 2u * pc + 1u)) = b.u;
                     } else {
@@ -528,12 +555,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                             part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].x, kr[n * NK + j].y, 0x3c00u), qr[2 * j].v, part[j], 0, 0, 0);
                             part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].z, kr[n * NK + j].w, 0x3c00u), qr[2 * j + 1].v, part[j], 0, 0, 0);
                         }
+                        const uint4 k4 = *(const uint4 *)&scales[wave][0][16u * n + 4u * gr], v4 = *(const uint4 *)&scales[wave][1][16u * n + 4u * gr];
+                        const u32 ks[4] = {k4.x, k4.y, k4.z, k4.w}, vs[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
                         for (u32 i = 0; i < 4; ++i) {
-                            const u32 s2 = (u32)__shfl((int)ksc, (int)(16u * n + 4u * gr + i));
-                            float v = part[0][i] * (float)__builtin_bit_cast(h16, (unsigned short)(s2 & 0xffffu));
-                            if (D == 128) v = fmaf(part[D / 64 - 1][i], (float)__builtin_bit_cast(h16, (unsigned short)(s2 >> 16)), v);
+                            float v = part[0][i] * scale_of(ks[i], 0);
+                            if (D == 128) v = fmaf(part[D / 64 - 1][i], scale_of(ks[i], 1), v);
                             sc[4 * n + i] = v;
+                            sv[4 * n + i] = vs[i];
                         }
                     } else {
                         f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -573,12 +602,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                     for (u32 i = 0; i < 4; ++i) o[n][i] *= corr;
             }
             const float mc = m == -INFINITY ? 0.0f : m * g.c;
-            U4H8 p;
+            constexpr u32 NP = Q8 ? D / 64 : 1;
+            U4H8 p[NP];
 #pragma unroll
             for (u32 i = 0; i < 8; ++i) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -mc));
                 l += e;
-                p.h[i] = (h16)e;
+#pragma unroll
+                for (u32 j = 0; j < NP; ++j) p[j].h[i] = Q8 ? (h16)(e * (scale_of(sv[i], j) * unit)) : (h16)e;
             }
 #pragma unroll
             for (u32 n = 0; n < D / 16; ++n) {
@@ -594,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                 const uint2 a0 = tr(key), a1 = tr(key + 16u);
                 U4H8 vv;
                 vv.u = make_uint4(a0.x, a0.y, a1.x, a1.y);
-                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv.v, p.v, o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv.v, p[Q8 ? n / 4u : 0u].v, o[n], 0, 0, 0);
             }
         }
         l += __shfl_xor(l, 16);
@@ -602,7 +633,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
         /* the four states: lane holds head col, dims 16 n + 4 gr + i */
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (u32 n = 0; n < D / 16; ++n) *(f32x4 *)(vt + (col * ORS + 16u * n + 4u * gr) * 4u) = o[n];
+        for (u32 n = 0; n < D / 16; ++n) {
+            if constexpr (Q8) {
+#pragma unroll
+                for (u32 i = 0; i < 4; ++i) o[n][i] *= 1.0f / unit;
+            }
+            *(f32x4 *)(vt + (col * ORS + 16u * n + 4u * gr) * 4u) = o[n];
+        }
         if (lane < 16u) {
             sml[wave][0][col] = m;
             sml[wave][1][col] = l;
@@ -643,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
             const uint64_t T0 = base + (uint64_t)set * ntp;
             const u32 b0 = block_of(sp, T0), b1 = block_of(sp, T0 + ntp - 1u);
             if (t == 0u) {
-                u32 *count = g.count + (uint64_t)s * sets + set;
+                u32 *count = g.count + b0;
                 arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (arrived == b1 - b0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
@@ -714,15 +751,9 @@ hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
     return hipGetLastError();
 }
 
-namespace {
-size_t partial_bytes(u32 rows, u32 dim) {
-    return (size_t)2u * PA_BLOCKS * rows * (dim + 4u) * sizeof(float);
-}
-}  // namespace
-
-size_t uocr_paged_attention_ws_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
-    const u32 group = heads / kv_heads, chunks = (group + 15u) / 16u;
-    return partial_bytes(group < 16u ? group : 16u, dim) + (size_t)n_seqs * kv_heads * chunks * sizeof(u32);
+size_t uocr_paged_attention_ws_bytes(uint32_t heads, uint32_t kv_heads, uint32_t dim) {
+    const u32 group = heads / kv_heads, rows = group < 16u ? group : 16u;
+    return PA_BLOCKS * sizeof(u32) + (size_t)2u * PA_BLOCKS * rows * (dim + 4u) * sizeof(float);
 }
 
 hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a) {
@@ -732,7 +763,8 @@ hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a)
     g.chunks = (g.group + 15u) / 16u;
     g.rows = g.group < 16u ? g.group : 16u;
     g.c = a->scale * 1.4426950408889634f;
-    g.count = (u32 *)((uint8_t *)a->part + partial_bytes(g.rows, a->kv.dim));
+    g.count = (u32 *)a->part;
+    g.a.part = a->part + PA_BLOCKS;
     /* A set has at most PA_BLOCKS / sets + 2 partials (all sets of a sequence have as many tiles).  One block reads them
      * one after another, the launch of its own with a block for each head: that pays where they are many. */
     g.fused = (PA_BLOCKS / (a->kv.heads * g.chunks) + 2u) * g.rows <= FUSED_ROWS;

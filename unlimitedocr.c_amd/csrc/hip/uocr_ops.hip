@@ -780,7 +780,7 @@ extern "C" size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint3
         heads % kv_heads != 0u || (head_dim != 64u && head_dim != 128u)) {
         return 0u;
     }
-    return uocr_paged_attention_ws_bytes(n_seqs, heads, kv_heads, head_dim);
+    return uocr_paged_attention_ws_bytes(heads, kv_heads, head_dim);
 }
 
 extern "C" int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_t *lengths, uint32_t heads,

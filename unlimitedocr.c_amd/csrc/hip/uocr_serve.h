@@ -81,7 +81,7 @@ struct uocr_sample_args {
 
 hipError_t uocr_launch_kv_append(hipStream_t st, const uocr_append_args *a);
 hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a);
-size_t uocr_paged_attention_ws_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads, uint32_t dim);
+size_t uocr_paged_attention_ws_bytes(uint32_t heads, uint32_t kv_heads, uint32_t dim);
 hipError_t uocr_launch_paged_attention(hipStream_t st, const uocr_paged_args *a);
 hipError_t uocr_launch_packed_attention(hipStream_t st, const uocr_packed_args *a);
 size_t uocr_sample_ws_bytes(uint32_t rows, uint32_t vocab);
