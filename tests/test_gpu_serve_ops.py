@@ -525,6 +525,33 @@ def test_sample_mixed_rows(gpu):
                 p=rng.choice([1.0, 0.9, 0.2], rows), m=rng.choice([0.0, 0.05], rows), u=rng.uniform(0, 1, rows))
 
 
+@pytest.mark.parametrize("f32", [False, True], ids=["f16", "f32"])
+def test_sample_long_crowded_rows(gpu, f32):
+    """Few different values in rows that several blocks share."""
+    rng = np.random.default_rng(25)
+    x = rng.integers(0, 3, (8, 40001)).astype(np.float32)
+    u = rng.uniform(0, 1, 8)
+    for s in (dict(k=100), dict(p=0.37), dict(k=4000, p=0.77), dict(k=40000), dict(t=5.0, p=0.5), dict(t=1e6, p=0.613), dict(m=0.2), dict(m=1.0)):
+        sample_case(gpu, x, f32, u=u, **s)
+    x[:, ::7] = -np.inf
+    x[1, :] = 2.0
+    x[2, 1:] = np.nan
+    x[3, ::2] = np.inf
+    x[4] = -np.inf
+    x[4, 39999] = 1.0
+    x[5] = -np.inf
+    for s in (dict(), dict(k=1024), dict(k=1025, p=0.9), dict(p=0.999), dict(t=0.0), dict(t=float("inf"), k=30000, p=0.51)):
+        sample_case(gpu, x, f32, u=u, **s)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 16384), (1, 16385), (64, 32768), (64, 32769), (63, 20000), (2, 300007), (1, 1500000)])
+def test_sample_one_block_or_several(gpu, rows, vocab):
+    """Sizes on both sides of where rows are shared, rows of more than 512 steps, each row with settings of its own."""
+    rng = np.random.default_rng(rows + vocab)
+    sample_case(gpu, rng.standard_normal((rows, vocab)) * 3, True, t=rng.choice([0.6, 1.0, 1.3], rows), k=rng.choice([0, 30, 700], rows),
+                p=rng.choice([1.0, 0.9, 0.5], rows), m=rng.choice([0.0, 0.01], rows), u=rng.uniform(0, 1, rows), gap=5)
+
+
 # ---- together -------------------------------------------------------------------------------
 
 def test_prompts_then_decode(gpu):

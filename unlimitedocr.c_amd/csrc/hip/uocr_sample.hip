@@ -12,13 +12,15 @@ namespace {
 
 constexpr u32 NT = 1024, WAVES = NT / 64; /* a block that has a row of its own */
 constexpr u32 CT = 512, CWAVES = CT / 64; /* a block that has a part of a row */
+constexpr u32 ROW_U = 1;                  /* steps that it loads at a time: its registers hold no more */
 constexpr u32 E = 8, STEP = 64 * E;       /* values of a lane and of a wavefront per step */
 constexpr u32 BINS = 2048;
-constexpr u32 LIST = 1024;                /* values that are ordered by comparing all pairs */
+constexpr u32 LIST = 1024;                /* values that are ordered at once, one a thread */
 constexpr u32 GROUPS = 64;                /* partial sums of a wavefront's run in the last pass */
 constexpr u32 IDX_BITS = 24, IDX_MASK = (1u << IDX_BITS) - 1u;
 constexpr u32 TAB = 1024;                 /* 2^(i / TAB) */
 constexpr u32 MAX_CHUNKS = 64;
+constexpr u32 TOPS = 512;                 /* groups of steps whose largest logits bound top-k */
 
 /* Weights are integers in units of 2^-shift, shift = 62 - log2(vocab) rounded
  * up (50 at most): their sums neither overflow nor depend on the order of
@@ -66,8 +68,25 @@ __device__ __forceinline__ double weight(const Row &r, const double *tab, float 
 __device__ __forceinline__ u64 units(double w) {
     return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
 }
+
+/* 2^(i / TAB) by the exponential series: 24 terms of at most ln 2 leave less than 2^-90. */
+struct Powers {
+    double v[TAB];
+};
+constexpr Powers powers() {
+    Powers p = {};
+    for (u32 i = 0; i < TAB; ++i) {
+        const double x = 0.6931471805599453 * i / TAB;
+        double sum = 1.0;
+        for (int n = 24; n > 0; --n) sum = 1.0 + x / n * sum;
+        p.v[i] = sum;
+    }
+    return p;
+}
+__device__ const Powers g_powers = powers();
+
 __device__ __forceinline__ void fill_table(double *tab) {
-    for (u32 i = threadIdx.x; i < TAB; i += blockDim.x) tab[i] = exp2((double)i / TAB);
+    for (u32 i = threadIdx.x; i < TAB; i += blockDim.x) tab[i] = g_powers.v[i];
 }
 
 /* Bins of equal width below the largest logit, over the range where a weight
@@ -99,11 +118,10 @@ __device__ __forceinline__ Row row_of(const uocr_sample_args &a, u32 b, u64 max_
     return r;
 }
 
-/* f(logit, id) for the E values of the lane at id0, those inside the row. */
-template <bool F32, typename F>
-__device__ __forceinline__ void lane_values(const void *row, u32 id0, u32 vocab, F &&f) {
-    float x[E];
-    if (id0 + E <= vocab) {
+/* The E values of the lane at id0; NaN, which takes part in nothing, outside the row. */
+template <bool F32, bool INSIDE>
+__device__ __forceinline__ void lane_load(const void *row, u32 id0, u32 vocab, float *x) {
+    if (INSIDE || id0 + E <= vocab) {
         if constexpr (F32) {
             const f32x4_any4 a = *(const f32x4_any4 *)((const float *)row + id0), b = *(const f32x4_any4 *)((const float *)row + id0 + 4);
             x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
@@ -116,21 +134,70 @@ __device__ __forceinline__ void lane_values(const void *row, u32 id0, u32 vocab,
 #pragma unroll
             for (u32 e = 0; e < E; ++e) x[e] = (float)v.h[e];
         }
-#pragma unroll
-        for (u32 e = 0; e < E; ++e) f(x[e], id0 + e);
     } else {
-        for (u32 id = id0; id < vocab; ++id) f(F32 ? ((const float *)row)[id] : (float)((const _Float16 *)row)[id], id);
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) x[e] = id0 + e >= vocab ? __builtin_nanf("") : F32 ? ((const float *)row)[id0 + e] : (float)((const _Float16 *)row)[id0 + e];
     }
+}
+__device__ __forceinline__ float largest_of(const float *x) {
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+}
+
+/* f(step, values) for the steps s0, s0 + stride, .. below s1, by a wavefront:
+ * U steps' loads at a time, or a pass over a row would be a chain of
+ * memory latencies. */
+template <bool F32, u32 U, typename F>
+__device__ __forceinline__ void each_step(const void *row, u32 vocab, u32 s0, u32 s1, u32 stride, F &&f) {
+    const u32 lane = threadIdx.x & 63u;
+    u32 s = s0;
+    if constexpr (U > 1)
+    for (; s + (U - 1u) * stride < s1 && (s + (U - 1u) * stride + 1u) * STEP <= vocab; s += U * stride) {
+        float x[U][E];
+#pragma unroll
+        for (u32 u = 0; u < U; ++u) lane_load<F32, true>(row, (s + u * stride) * STEP + lane * E, vocab, x[u]);
+#pragma unroll
+        for (u32 u = 0; u < U; ++u) f(s + u * stride, x[u]);
+    }
+    for (; s < s1; s += stride) {
+        float x[E];
+        lane_load<F32, false>(row, min(s * STEP + lane * E, vocab), vocab, x);
+        f(s, x);
+    }
+}
+
+/* g(logit, id) for the lane's values of step s that are at least `least` (not
+ * NaN): few lanes have one where few values are kept. */
+template <typename G>
+__device__ __forceinline__ void values_from(float least, u32 s, const float *x, G &&g) {
+    if (!(largest_of(x) >= least)) return;
+    const u32 id0 = s * STEP + (threadIdx.x & 63u) * E;
+#pragma unroll
+    for (u32 e = 0; e < E; ++e)
+        if (x[e] >= least) g(x[e], id0 + e);
+}
+
+/* The step's largest logit, in every lane; best and best_id of the lane. */
+__device__ __forceinline__ float step_largest(u32 s, const float *x, float &best, u32 &best_id) {
+    float m = largest_of(x);
+    if (m > best) {
+        best = m;
+        const u32 id0 = s * STEP + (threadIdx.x & 63u) * E;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) best_id = x[e] == m ? id0 + e : best_id;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m;
 }
 
 __device__ __forceinline__ float value_of(const Row &r, float x) {
     return !r.inf ? x : x == INFINITY ? 0.0f : -INFINITY;
 }
 
-/* f over the whole row, by all threads. */
+/* f over the whole row's values from `least` on, by all threads. */
 template <bool F32, typename F>
-__device__ __forceinline__ void row_values(const void *row, u32 vocab, F &&f) {
-    for (u32 id0 = threadIdx.x * E; id0 < vocab; id0 += NT * E) lane_values<F32>(row, id0, vocab, f);
+__device__ __forceinline__ void row_values(const void *row, u32 vocab, float least, F &&f) {
+    each_step<F32, ROW_U>(row, vocab, threadIdx.x >> 6, (vocab + STEP - 1u) / STEP, WAVES, [&](u32 s, const float *x) { values_from(least, s, x, f); });
 }
 
 __device__ __forceinline__ u64 shfl64(u64 v, int src) {
@@ -161,7 +228,7 @@ struct Shared {
     u64 weight[BINS];
     u32 count[BINS];
     u64 list[LIST];
-    u64 list_w[LIST];
+    u32 tops[TOPS], place[512];
     u64 red[WAVES];
     u64 red2[WAVES];
     u64 out[4];
@@ -181,6 +248,96 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *red, u64 &all) {
     }
     __syncthreads();
     return before;
+}
+
+/* The ranks of the block's LIST threads, largest first; the first n threads have
+ * one, the others 0.  Few are counted against each other, by all threads (256:
+ * 1 us); from about 400 on a bitonic sort, by lane exchange within wavefronts,
+ * is the faster one (7 us). */
+__device__ __forceinline__ u64 sorted(u64 rank, u32 n, u64 *buf, u32 *place) {
+    const u32 t = threadIdx.x;
+    u32 size = 64u;
+    while (size < n) size <<= 1;
+    if (n <= 384u) {
+        const u32 parts = LIST / size, part = t / size, e = t % size;
+        if (t < size) {
+            buf[t] = rank;
+            place[t] = 0u;
+        }
+        __syncthreads();
+        if (e < n) {
+            const u64 mine = buf[e];
+            const u32 i1 = n * (part + 1u) / parts;
+            u32 before = 0;
+#pragma unroll 4
+            for (u32 i = n * part / parts; i < i1; ++i) before += buf[i] > mine ? 1u : 0u;
+            if (before != 0u) atomicAdd(&place[e], before);
+        }
+        __syncthreads();
+        if (t < n) buf[place[t]] = rank;
+        __syncthreads();
+        rank = t < n ? buf[t] : 0ull;
+        __syncthreads();
+        return rank;
+    }
+    for (u32 k = 2u; k <= size; k <<= 1) {
+        for (u32 j = k >> 1; j > 0u; j >>= 1) {
+            u64 other;
+            if (j >= 64u) {
+                buf[t] = rank;
+                __syncthreads();
+                other = buf[t ^ j];
+                __syncthreads();
+            } else {
+                other = shfl_xor64(rank, (int)j);
+            }
+            /* the lower place of a pair keeps the larger value in runs that descend */
+            const bool larger = ((t & j) == 0u) == ((t & k) == 0u);
+            rank = (other > rank) == larger ? other : rank;
+        }
+    }
+    return rank;
+}
+
+/* Top-k of up to 7/8 of the groups: k values are at least the k-th largest of
+ * the groups' largest, so what is below cannot be kept. */
+__device__ __forceinline__ bool bounded(const Row &r, u32 groups) {
+    return r.use_k && r.k <= groups * 7u / 8u;
+}
+/* tops[i] of lane l: group 64 i + l's, 0 where there is none; by each wavefront
+ * for itself, from the key's highest bit on.  To 20 bits: a bound may be lower. */
+template <u32 N>
+__device__ __forceinline__ u32 kth_key(const u32 *tops, u32 k) {
+    u32 key = 0;
+    for (u32 bit = 1u << 31; bit >= 1u << 12; bit >>= 1) {
+        u32 n = 0;
+#pragma unroll
+        for (u32 i = 0; i < N; ++i) n += (u32)__popcll(__ballot(tops[i] >= (key | bit)));
+        if (n >= k) key |= bit;
+    }
+    return key;
+}
+__device__ __forceinline__ float kth_largest(const u32 *tops, u32 groups, u32 k) {
+    const u32 key = groups <= 64u ? kth_key<1>(tops, k) : groups <= 256u ? kth_key<4>(tops, k) : kth_key<TOPS / 64>(tops, k);
+    return of_key(max(key, key_of(-INFINITY)));
+}
+
+/* The rank of the last value that is kept, of the n listed ones in order (one a
+ * thread), in front of which base_n values and base_w units stand; all: units
+ * of all values that top-p sums. */
+__device__ __forceinline__ u64 cut(const Row &r, const double *tab, u64 rank, u32 n, bool use_k, u64 base_n, u64 base_w, u64 all, u64 *red, u64 *out) {
+    const u32 t = threadIdx.x;
+    const bool in = t < n;
+    const u64 bn = base_n + t, w = in ? units(weight(r, tab, of_key((u32)(rank >> IDX_BITS)))) : 0ull;
+    const bool in_k = in && (!use_k || bn < r.k);
+    u64 sum;
+    const u64 bw = base_w + block_before(in_k ? w : 0ull, red, sum);
+    const double target = (double)r.p * (double)(use_k ? sum : all);
+    const bool kept = in_k && (!r.use_p || bn == 0ull || (double)bw < target);
+    const u32 last = (u32)__syncthreads_count(kept);
+    if (t + 1u == last) *out = rank;
+    __syncthreads();
+    return *out;
 }
 
 /* What is known of the value that ends a kept set: it lies in bin `bin`, its
@@ -210,7 +367,7 @@ __device__ u64 last_kept(const void *row, u32 vocab, const Row &r, Region g, dou
         const u32 sh = g.sh == 64u ? 45u : g.sh > 11u ? g.sh - 11u : 0u;
         for (u32 i = t; i < BINS; i += NT) sm.weight[i] = 0ull, sm.count[i] = 0u;
         __syncthreads();
-        row_values<F32>(row, vocab, [&](float raw, u32 id) {
+        row_values<F32>(row, vocab, -INFINITY, [&](float raw, u32 id) {
             const float x = value_of(r, raw);
             const u64 rank = rank_of(x, id);
             if (!inside(x, rank)) return;
@@ -240,55 +397,47 @@ __device__ u64 last_kept(const void *row, u32 vocab, const Row &r, Region g, dou
     }
     if (t == 0u) sm.n = 0u;
     __syncthreads();
-    row_values<F32>(row, vocab, [&](float raw, u32 id) {
+    row_values<F32>(row, vocab, -INFINITY, [&](float raw, u32 id) {
         const float x = value_of(r, raw);
         const u64 rank = rank_of(x, id);
         if (!inside(x, rank)) return;
-        const u32 at = atomicAdd(&sm.n, 1u);
-        sm.list[at] = rank;
-        sm.list_w[at] = units(weight(r, sm.tab, x));
+        sm.list[atomicAdd(&sm.n, 1u)] = rank;
     });
     __syncthreads();
     const u32 n = sm.n;
-    u64 mine = ~0ull, w = 0;
-    if (t < n) {
-        const u64 rank = sm.list[t];
-        u64 before = g.before;
-        for (u32 i = 0; i < n; ++i)
-            if (sm.list[i] > rank) before += WEIGHTED ? sm.list_w[i] : 1ull;
-        if ((double)before < limit) mine = rank, w = sm.list_w[t];
-    }
-    u64 sum;
-    (void)block_before(w, sm.red, sum);
-    kept_w += sum;
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 v = shfl_xor64(mine, o);
-        mine = v < mine ? v : mine;
-    }
-    if ((t & 63u) == 0u) sm.red[t >> 6] = mine;
+    const u64 rank = sorted(t < n ? sm.list[t] : 0ull, n, sm.list, sm.place);
+    const u64 w = t < n ? units(weight(r, sm.tab, of_key((u32)(rank >> IDX_BITS)))) : 0ull;
+    u64 all;
+    const u64 before = g.before + block_before(t >= n ? 0ull : WEIGHTED ? w : 1ull, sm.red, all);
+    const bool kept = t < n && (double)before < limit;
+    (void)block_before(kept ? w : 0ull, sm.red, all);
+    kept_w += all;
+    const u32 last = (u32)__syncthreads_count(kept);
+    if (t + 1u == last) sm.out[0] = rank;
     __syncthreads();
-    for (u32 i = 0; i < WAVES; ++i) mine = sm.red[i] < mine ? sm.red[i] : mine;
+    const u64 thr = sm.out[0];
     __syncthreads();
-    return mine;
+    return thr;
 }
 
-/* The first id whose running sum of kept units is over the target, in the
- * STEP values from id0 in front of which `sum` stands; by one wavefront.
+/* The first id whose running sum of kept units is over the target, in the step
+ * that `sum` stands in front of; by one wavefront.
  * Returns whether it is there, and what stands in front of the next values. */
 template <bool F32, typename K>
-__device__ __forceinline__ bool pick(const uocr_sample_args &a, u32 b, const void *row, u32 id0, double target, u64 all, u64 &sum, K &&kept) {
+__device__ __forceinline__ bool pick(const uocr_sample_args &a, u32 b, const void *row, u32 step, float least, double target, u64 all, u64 &sum, K &&kept) {
     const u32 lane = threadIdx.x & 63u;
-    id0 = min(id0 + lane * E, a.vocab);
+    float x[E];
+    lane_load<F32, false>(row, min(step * STEP + lane * E, a.vocab), a.vocab, x);
     u64 s = 0;
-    lane_values<F32>(row, id0, a.vocab, [&](float x, u32 id) { s += kept(x, id); });
+    values_from(least, step, x, [&](float v, u32 id) { s += kept(v, id); });
     u64 at = sum + wave_before(s);
     const u64 found = __ballot(s != 0ull && !((double)at > target) && (double)(at + s) > target);
     sum = shfl64(at + s, 63);
     if (found == 0ull) return false;
     if (lane == (u32)__ffsll((long long)found) - 1u) {
         bool done = false;
-        lane_values<F32>(row, id0, a.vocab, [&](float x, u32 id) {
-            const u64 v = kept(x, id);
+        values_from(least, step, x, [&](float y, u32 id) {
+            const u64 v = kept(y, id);
             at += v;
             if (!done && v != 0ull && (double)at > target) {
                 done = true;
@@ -319,14 +468,8 @@ __device__ __forceinline__ float temperature_of(const uocr_sample_args &a, u32 b
     return a.temperature != nullptr ? a.temperature[b] : 1.0f;
 }
 
-/* The largest logit's rank, of the values that `each` goes over. */
-template <typename G>
-__device__ __forceinline__ u64 largest(u64 *red, G &&each) {
-    float best = -INFINITY;
-    u32 best_id = 0xffffffffu;
-    each([&](float x, u32 id) {
-        if (x > best) best = x, best_id = id;
-    });
+/* The rank of the block's largest logit, from its lanes'. */
+__device__ __forceinline__ u64 largest(float best, u32 best_id, u64 *red) {
     u64 rank = best_id == 0xffffffffu ? 0ull : rank_of(best, best_id);
     for (int o = 32; o > 0; o >>= 1) {
         const u64 v = shfl_xor64(rank, o);
@@ -341,33 +484,66 @@ __device__ __forceinline__ u64 largest(u64 *red, G &&each) {
 
 /* Units that a value brings to the kept sum: ranks from thr on, not below min_p. */
 __device__ __forceinline__ u64 kept_units(const Row &r, const double *tab, float least, u64 thr, float x, u32 id) {
-    if (!(x >= least) || (x == least && rank_of(x, id) < thr)) return 0ull;
+    if (x == least && rank_of(x, id) < thr) return 0ull;
     const double w = weight(r, tab, x);
     return w >= r.min_w ? units(w) : 0ull;
 }
-/* The logit below which nothing is kept. */
+/* The logit below which nothing is kept (with +inf ones, as they stand in the
+ * row: those alone). */
 __device__ __forceinline__ float least_of(const Row &r, u64 thr) {
     return thr == 0ull ? r.cut : fmaxf(r.cut, of_key((u32)(thr >> IDX_BITS)));
 }
+__device__ __forceinline__ float least_raw(const Row &r, float least) {
+    return r.inf ? INFINITY : least;
+}
 
-/* A row in one block (max_rank: 0 where it is not known yet).  The kept set of
- * top-k and top-p is all values from some rank on: a histogram over bins below
- * the maximum (counts, and units of weight for top-p) finds the bin of the last
- * kept value, the bin's few values are then ordered by comparing them. */
+/* A row in one block.  The kept set of top-k and top-p is all values from some
+ * rank on.  For a small k the values that can be in it are those from the k-th
+ * largest of 512-value steps' maxima on, some k to 2 k of them, which are listed
+ * and ordered.  Else a histogram over bins below the maximum (counts, and units
+ * of weight for top-p) finds the bin of the last kept value, and the bin's few
+ * values are ordered. */
 template <bool F32>
 __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32 shift, Shared &sm) {
     const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, vocab = a.vocab;
-    const u64 max_rank = largest(sm.red, [&](auto f) { row_values<F32>(row, vocab, f); });
+    const u32 steps = (vocab + STEP - 1u) / STEP, groups = min(steps, TOPS);
+    float best = -INFINITY;
+    u32 best_id = 0xffffffffu;
+    sm.tops[t % TOPS] = 0u;
+    __syncthreads();
+    each_step<F32, ROW_U>(row, vocab, wave, steps, WAVES, [&](u32 s, const float *x) {
+        const u32 top = key_of(step_largest(s, x, best, best_id));
+        if (lane == 0u) sm.tops[s % TOPS] = max(sm.tops[s % TOPS], top); /* a group's steps are one wavefront's: TOPS is a multiple of WAVES */
+    });
+    const u64 max_rank = largest(best, best_id, sm.red);
     const float temp = temperature_of(a, b);
     if (greedy(a, b, max_rank, temp)) return;
     const Row r = row_of(a, b, max_rank, temp, shift);
     fill_table(sm.tab);
+    if (t == 0u) sm.n = 0u;
+    __syncthreads();
 
     u64 thr = 0; /* kept: ranks from here on */
-    if (r.use_k || r.use_p) {
+    bool found = false;
+    if (bounded(r, groups)) {
+        u32 tops[TOPS / 64];
+#pragma unroll
+        for (u32 i = 0; i < TOPS / 64; ++i) tops[i] = sm.tops[64u * i + lane];
+        const float floor = kth_largest(tops, groups, r.k);
+        row_values<F32>(row, vocab, floor, [&](float raw, u32 id) {
+            const u32 at = atomicAdd(&sm.n, 1u);
+            if (at < LIST) sm.list[at] = rank_of(value_of(r, raw), id);
+        });
+        __syncthreads();
+        const u32 n = sm.n;
+        found = n <= LIST;
+        if (found) thr = cut(r, sm.tab, sorted(t < n ? sm.list[t] : 0ull, n, sm.list, sm.place), n, true, 0ull, 0ull, 0ull, sm.red, &sm.out[0]);
+        __syncthreads();
+    }
+    if (!found && (r.use_k || r.use_p)) {
         for (u32 i = t; i < BINS; i += NT) sm.weight[i] = 0ull, sm.count[i] = 0u;
         __syncthreads();
-        row_values<F32>(row, vocab, [&](float raw, u32 id) {
+        row_values<F32>(row, vocab, -INFINITY, [&](float raw, u32 id) {
             const float x = value_of(r, raw);
             const u32 i = bin_of(r, x);
             if (i == BINS - 1u) return; /* no weight */
@@ -408,20 +584,20 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
     }
 
     /* the kept weights by id: a run of the row for each wavefront, a sum for each group of its steps */
-    const u32 steps = (vocab + STEP - 1u) / STEP, run = (steps + WAVES - 1u) / WAVES, per = (run + GROUPS - 1u) / GROUPS;
-    const float least = least_of(r, thr);
+    const u32 run = (steps + WAVES - 1u) / WAVES, per = (run + GROUPS - 1u) / GROUPS;
+    const float least = least_of(r, thr), raw_least = least_raw(r, least);
     auto kept = [&](float raw, u32 id) { return kept_units(r, sm.tab, least, thr, value_of(r, raw), id); };
     u64 *sums = sm.weight; /* [WAVES][GROUPS] */
     __syncthreads();
     sums[t] = 0ull;
     __syncthreads();
-    for (u32 g = 0; g * per < run; ++g) {
-        u64 s = 0;
-        for (u32 i = g * per; i < min(g * per + per, run); ++i)
-            lane_values<F32>(row, min((wave * run + i) * STEP + lane * E, vocab), vocab, [&](float x, u32 id) { s += kept(x, id); });
-        s = wave_sum64(s);
-        if (lane == 0u) sums[wave * GROUPS + g] = s;
-    }
+    each_step<F32, ROW_U>(row, vocab, min(wave * run, steps), min(wave * run + run, steps), 1u, [&](u32 s, const float *x) {
+        u64 sum = 0;
+        values_from(raw_least, s, x, [&](float v, u32 id) { sum += kept(v, id); });
+        if (!__any(sum != 0ull)) return;
+        sum = wave_sum64(sum);
+        if (lane == 0u) sums[wave * GROUPS + (s - wave * run) / per] += sum;
+    });
     __syncthreads();
     const u64 mine = sums[t];
     u64 all;
@@ -434,7 +610,7 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
         const u32 w = (u32)sm.out[0] / GROUPS, g = (u32)sm.out[0] % GROUPS;
         u64 sum = sm.out[1];
         for (u32 i = g * per; i < min(g * per + per, run); ++i)
-            if (pick<F32>(a, b, row, min((w * run + i) * STEP, vocab), target, all, sum, kept)) break;
+            if (w * run + i < steps && pick<F32>(a, b, row, w * run + i, raw_least, target, all, sum, kept)) break;
     }
 }
 
@@ -452,18 +628,19 @@ __global__ __launch_bounds__(NT) void k_sample_row(uocr_sample_args a, u32 shift
 /* ---- a row over several blocks --------------------------------------------------- */
 
 /* What the histogram says of a row: whether its kept set ends (any), in a list
- * of n values that base_n values and base_w units stand in front of; crowded
- * lists are not made. */
+ * of n values that base_n values and base_w units stand in front of. */
 struct Found {
     u64 base_n, base_w, all_w;
-    u32 n, any, use_k, crowded;
+    u32 n, any, use_k, pad;
 };
 
 /* What the launches of a row leave for each other, in the workspace. */
 struct Plan {
     uocr_sample_args a;
-    u32 shift, steps, chunks, run; /* of a row; run: steps of a chunk */
+    u32 shift, steps, chunks;      /* of a row; chunks: of the first launch */
+    u32 parts, run;                /* of this launch: blocks of a row, steps of each */
     u64 *max_rank;                 /* [rows][chunks] */
+    u32 *tops;                     /* [rows][steps]: keys of the steps' largest logits */
     u64 *weight;                   /* [rows][BINS] */
     u32 *count;                    /* [rows][BINS] */
     u64 *list;                     /* [rows][LIST] */
@@ -475,24 +652,33 @@ struct Plan {
 };
 
 template <bool F32, typename F>
-__device__ __forceinline__ void chunk_values(const Plan &g, const void *row, u32 chunk, F &&f) {
-    const u32 s1 = min(chunk * g.run + g.run, g.steps);
-    for (u32 s = chunk * g.run + (threadIdx.x >> 6); s < s1; s += CWAVES)
-        lane_values<F32>(row, min(s * STEP + (threadIdx.x & 63u) * E, g.a.vocab), g.a.vocab, f);
+__device__ __forceinline__ void chunk_steps(const Plan &g, const void *row, u32 chunk, F &&f) {
+    each_step<F32, 4>(row, g.a.vocab, chunk * g.run + (threadIdx.x >> 6), min(chunk * g.run + g.run, g.steps), CWAVES, f);
+}
+template <bool F32, typename F>
+__device__ __forceinline__ void chunk_values(const Plan &g, const void *row, u32 chunk, float least, F &&f) {
+    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) { values_from(least, s, x, f); });
 }
 
-/* 1: the chunk's largest logit; the row's histogram is cleared. */
+/* 1: the steps' and the chunk's largest logit; the row's histogram is cleared. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_max(Plan g) {
     __shared__ u64 red[CWAVES];
-    const u32 b = blockIdx.x / g.chunks, chunk = blockIdx.x % g.chunks;
-    for (u32 i = chunk * CT + threadIdx.x; i < BINS; i += CT * g.chunks) g.weight[(u64)b * BINS + i] = 0ull, g.count[(u64)b * BINS + i] = 0u;
+    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, lane = threadIdx.x & 63u;
+    if (g.cut)
+        for (u32 i = chunk * CT + threadIdx.x; i < BINS; i += CT * g.parts) g.weight[(u64)b * BINS + i] = 0ull, g.count[(u64)b * BINS + i] = 0u;
     if (chunk == 0u && threadIdx.x == 0u) {
         g.n[b] = 0u;
         g.found[b] = Found{};
     }
     const void *row = row_at<F32>(g.a, b);
-    const u64 rank = largest(red, [&](auto f) { chunk_values<F32>(g, row, chunk, f); });
+    float best = -INFINITY;
+    u32 best_id = 0xffffffffu;
+    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) {
+        const float top = step_largest(s, x, best, best_id);
+        if (lane == 0u) g.tops[(u64)b * g.steps + s] = key_of(top);
+    });
+    const u64 rank = largest(best, best_id, red);
     if (threadIdx.x == 0u) g.max_rank[(u64)b * g.chunks + chunk] = rank;
 }
 
@@ -511,16 +697,16 @@ __global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
     __shared__ double tab[TAB];
     __shared__ u64 weights[BINS];
     __shared__ u32 counts[BINS];
-    const u32 b = blockIdx.x / g.chunks, chunk = blockIdx.x % g.chunks;
+    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts;
     const u64 max_rank = row_max(g, b);
     const float temp = temperature_of(g.a, b);
     if (max_rank == 0ull || !(temp > 0.0f)) return;
     const Row r = row_of(g.a, b, max_rank, temp, g.shift);
-    if (!r.use_k && !r.use_p) return;
+    if ((!r.use_k && !r.use_p) || bounded(r, min(g.steps, TOPS))) return;
     for (u32 i = threadIdx.x; i < BINS; i += CT) weights[i] = 0ull, counts[i] = 0u;
     if (r.use_p) fill_table(tab);
     __syncthreads();
-    chunk_values<F32>(g, row_at<F32>(g.a, b), chunk, [&](float raw, u32 id) {
+    chunk_values<F32>(g, row_at<F32>(g.a, b), chunk, -INFINITY, [&](float raw, u32 id) {
         const float x = value_of(r, raw);
         const u32 i = bin_of(r, x);
         if (i == BINS - 1u) return;
@@ -582,121 +768,118 @@ __device__ __forceinline__ Deciding deciding(const Plan &g, u32 b, const Row &r,
     return d;
 }
 
-/* 3: the values in the deciding bins, listed (in any order). */
+/* 3: the values that decide, listed (in any order): those from top-k's bound on,
+ * or those in the deciding bins. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_list(Plan g) {
     __shared__ u64 red[CWAVES], red2[CWAVES], out[4], list[LIST];
     __shared__ u32 n, first;
-    const u32 b = blockIdx.x / g.chunks, chunk = blockIdx.x % g.chunks;
+    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, t = threadIdx.x;
     const u64 max_rank = row_max(g, b);
     const float temp = temperature_of(g.a, b);
     if (max_rank == 0ull || !(temp > 0.0f)) return;
     const Row r = row_of(g.a, b, max_rank, temp, g.shift);
     if (!r.use_k && !r.use_p) return;
-    if (threadIdx.x == 0u) n = 0u;
-    const Deciding d = deciding(g, b, r, red, red2, out);
-    if (chunk == 0u && threadIdx.x == 0u) {
-        Found &f = g.found[b];
-        f.crowded = d.any && d.n > LIST ? 1u : 0u;
+    if (t == 0u) n = 0u;
+    const u32 groups = min(g.steps, TOPS);
+    const void *row = row_at<F32>(g.a, b);
+    Found f = {};
+    f.any = 1u;
+    if (bounded(r, groups)) {
+        u32 tops[TOPS / 64] = {};
+        for (u32 s0 = 0; s0 < g.steps; s0 += TOPS) {
+#pragma unroll
+            for (u32 i = 0; i < TOPS / 64; ++i) {
+                const u32 s = s0 + 64u * i + (t & 63u);
+                if (s < g.steps) tops[i] = max(tops[i], g.tops[(u64)b * g.steps + s]);
+            }
+        }
+        const float floor = kth_largest(tops, groups, r.k);
+        __syncthreads();
+        f.use_k = 1u;
+        f.n = LIST;
+        if (chunk == 0u && t == 0u) g.found[b] = f;
+        chunk_values<F32>(g, row, chunk, floor, [&](float raw, u32 id) {
+            const u32 at = atomicAdd(&n, 1u);
+            if (at < LIST) list[at] = rank_of(value_of(r, raw), id);
+        });
+    } else {
+        const Deciding d = deciding(g, b, r, red, red2, out);
         f.any = d.any ? 1u : 0u;
-        f.use_k = d.use_k ? 1u : 0u;
-        f.n = d.any ? d.n : 0u;
-        f.base_n = d.any ? d.base_n : 0ull;
-        f.base_w = d.any ? d.base_w : 0ull;
+        if (d.any) {
+            f.use_k = d.use_k ? 1u : 0u;
+            f.n = d.n;
+            f.base_n = d.base_n;
+            f.base_w = d.base_w;
+        }
         f.all_w = d.all_w;
+        if (chunk == 0u && t == 0u) {
+            g.found[b] = f;
+            if (d.any && d.n > LIST) g.n[b] = LIST + 1u; /* too many */
+        }
+        if (!d.any || d.n > LIST) return;
+        /* most values are well below the deciding bins: a comparison tells (three bins' margin for the bins' roundings) */
+        float floor = r.top - ((float)d.last + 3.0f) / r.scale;
+        if (!(floor > -INFINITY) || r.inf) floor = -INFINITY;
+        chunk_values<F32>(g, row, chunk, floor, [&](float raw, u32 id) {
+            const float x = value_of(r, raw);
+            const u32 i = bin_of(r, x);
+            if (i < d.first || i > d.last) return;
+            const u32 at = atomicAdd(&n, 1u);
+            if (at < LIST) list[at] = rank_of(x, id); /* at most d.n: the bins were counted by the same arithmetic */
+        });
     }
-    if (!d.any || d.n > LIST) return;
-    /* most values are well below the deciding bins: a comparison tells (two bins' margin for the bins' roundings) */
-    float floor = r.top - ((float)d.last + 3.0f) / r.scale;
-    if (!(floor > -INFINITY) || r.inf) floor = -INFINITY;
-    chunk_values<F32>(g, row_at<F32>(g.a, b), chunk, [&](float raw, u32 id) {
-        if (!(raw >= floor)) return;
-        const float x = value_of(r, raw);
-        const u32 i = bin_of(r, x);
-        if (i < d.first || i > d.last) return;
-        const u32 at = atomicAdd(&n, 1u);
-        if (at < LIST) list[at] = rank_of(x, id); /* at most d.n: the bins were counted by the same arithmetic */
-    });
     __syncthreads();
-    const u32 mine = min(n, LIST);
-    if (threadIdx.x == 0u && mine != 0u) first = atomicAdd(&g.n[b], mine);
+    if (t == 0u && n != 0u) first = atomicAdd(&g.n[b], n); /* of a crowded list: past LIST */
     __syncthreads();
-    for (u32 i = threadIdx.x; i < mine; i += CT)
+    for (u32 i = t; i < min(n, LIST); i += CT)
         if (first + i < LIST) g.list[(u64)b * LIST + first + i] = list[i];
 }
 
-/* 4: the rank that ends the kept set: the listed values in order (a bitonic
- * sort of one value a thread, by lane exchange within wavefronts), what stands
- * in front of each, and the last one that is kept. */
+/* 4: the rank that ends the kept set: the listed values in order, what stands in
+ * front of each, and the last one that is kept. */
 template <bool F32>
 __global__ __launch_bounds__(LIST) void k_sample_cut(Plan g) {
     __shared__ double tab[TAB];
-    __shared__ u64 red[LIST / 64], list[LIST];
+    __shared__ u64 red[LIST / 64], list[LIST], out;
+    __shared__ u32 place[512];
     const u32 b = blockIdx.x, t = threadIdx.x;
     const u64 max_rank = row_max(g, b);
     const float temp = temperature_of(g.a, b);
     if (max_rank == 0ull || !(temp > 0.0f)) return;
     const Row r = row_of(g.a, b, max_rank, temp, g.shift);
     const Found f = g.found[b];
-    if ((!r.use_k && !r.use_p) || f.any == 0u || f.crowded != 0u) {
-        if (t == 0u) g.thr[b] = 0ull;
-        return;
+    const u32 n = g.n[b];
+    u64 thr = 0;
+    if ((r.use_k || r.use_p) && f.any != 0u && n <= LIST) {
+        const u64 rank = t < n ? g.list[(u64)b * LIST + t] : 0ull;
+        fill_table(tab);
+        __syncthreads();
+        thr = cut(r, tab, sorted(rank, n, list, place), n, f.use_k != 0u, f.base_n, f.base_w, f.all_w, red, &out);
     }
-    u64 rank = t < f.n ? g.list[(u64)b * LIST + t] : 0ull; /* 0: behind all */
-    fill_table(tab);
-    __syncthreads();
-    u32 size = 64u;
-    while (size < f.n) size <<= 1;
-    for (u32 k = 2u; k <= size; k <<= 1) {
-        for (u32 j = k >> 1; j > 0u; j >>= 1) {
-            u64 other;
-            if (j >= 64u) {
-                list[t] = rank;
-                __syncthreads();
-                other = list[t ^ j];
-                __syncthreads();
-            } else {
-                other = shfl_xor64(rank, (int)j);
-            }
-            /* descending: the lower place of a pair keeps the larger value in runs that descend */
-            const bool larger = ((t & j) == 0u) == ((t & k) == 0u);
-            rank = (other > rank) == larger ? other : rank;
-        }
-    }
-    const bool in = t < f.n;
-    const u64 bn = f.base_n + t, w = in ? units(weight(r, tab, of_key((u32)(rank >> IDX_BITS)))) : 0ull;
-    const bool in_k = in && (f.use_k == 0u || bn < r.k);
-    u64 all;
-    const u64 bw = f.base_w + block_before(in_k ? w : 0ull, red, all);
-    if (!(f.use_k != 0u && r.use_p)) all = f.all_w;
-    const double target = (double)r.p * (double)all;
-    const bool kept = in_k && (!r.use_p || bn == 0ull || (double)bw < target);
-    const u32 n = (u32)__syncthreads_count(kept);
-    if (kept && t == n - 1u) g.thr[b] = rank;
+    if (t == 0u) g.thr[b] = thr;
 }
 
 /* 5: the kept units of each step. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_sums(Plan g) {
     __shared__ double tab[TAB];
-    const u32 b = blockIdx.x / g.chunks, chunk = blockIdx.x % g.chunks, t = threadIdx.x;
+    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, t = threadIdx.x;
     const u64 max_rank = row_max(g, b);
     const float temp = temperature_of(g.a, b);
-    if (max_rank == 0ull || !(temp > 0.0f) || (g.cut && g.found[b].crowded != 0u)) return;
+    if (max_rank == 0ull || !(temp > 0.0f) || (g.cut && g.n[b] > LIST)) return;
     const Row r = row_of(g.a, b, max_rank, temp, g.shift);
     const u64 thr = g.cut ? g.thr[b] : 0ull;
     fill_table(tab);
     __syncthreads();
     const void *row = row_at<F32>(g.a, b);
     const float least = least_of(r, thr);
-    const u32 s1 = min(chunk * g.run + g.run, g.steps);
-    for (u32 s = chunk * g.run + (t >> 6); s < s1; s += CWAVES) {
+    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) {
         u64 sum = 0;
-        lane_values<F32>(row, min(s * STEP + (t & 63u) * E, g.a.vocab), g.a.vocab,
-                         [&](float raw, u32 id) { sum += kept_units(r, tab, least, thr, value_of(r, raw), id); });
+        values_from(least_raw(r, least), s, x, [&](float raw, u32 id) { sum += kept_units(r, tab, least, thr, value_of(r, raw), id); });
         if (__any(sum != 0ull)) sum = wave_sum64(sum);
         if ((t & 63u) == 0u) g.sums[(u64)b * g.steps + s] = sum;
-    }
+    });
 }
 
 /* 6: the step that the target falls into, and its token.  Rows with crowded
@@ -709,7 +892,7 @@ __global__ __launch_bounds__(NT) void k_sample_pick(Plan g) {
     const u64 max_rank = row_max(g, b);
     const float temp = temperature_of(g.a, b);
     if (greedy(g.a, b, max_rank, temp)) return;
-    if (g.cut && g.found[b].crowded != 0u) {
+    if (g.cut && g.n[b] > LIST) {
         whole_row<F32>(g.a, b, row, g.shift, sm);
         return;
     }
@@ -729,7 +912,7 @@ __global__ __launch_bounds__(NT) void k_sample_pick(Plan g) {
     auto kept = [&](float raw, u32 id) { return kept_units(r, sm.tab, least, thr, value_of(r, raw), id); };
     u64 sum = sm.out[1];
     for (u32 s = (u32)sm.out[0]; s < g.steps; ++s)
-        if (pick<F32>(g.a, b, row, s * STEP, target, all, sum, kept)) break;
+        if (pick<F32>(g.a, b, row, s, least_raw(r, least), target, all, sum, kept)) break;
 }
 
 u32 shift_of(u32 vocab) {
@@ -738,17 +921,31 @@ u32 shift_of(u32 vocab) {
     return 62u - bits < 50u ? 62u - bits : 50u;
 }
 
-/* Rows of up to this many tokens are done by one block each, in one launch. */
-constexpr u32 ONE_BLOCK = 8192;
+/* Rows of up to ONE_BLOCK tokens are done by a block each, in one launch, and
+ * with MANY_ROWS or more up to twice that: us by one launch and by several, fp16,
+ * top-k alone and top-p alone, were 19 and 28 against 29 and 33 for 1 row of
+ * 16,000, 23 and 39 against 29 and 34 for 1 of 32,000, 34 and 48 against 38 and
+ * 47 for 64 of those, 49 and 80 against 55 and 80 for 192 of 64,000, 58 and 148
+ * against 64 and 124 for 192 of 129,280. */
+constexpr u32 ONE_BLOCK = 16384, MANY_ROWS = 64;
+bool by_one_block(u32 rows, u32 vocab) { return vocab <= (rows < MANY_ROWS ? ONE_BLOCK : 2u * ONE_BLOCK); }
+
+/* Blocks of a launch, all rows: where all values take little each, more of them
+ * only have their own beginnings to pay for; where some rows' values take an
+ * exponential and atomics each and others' nothing, the rows are cut finer.  192
+ * mixed rows of 129,280 fp16 took 93.9 us so, 95.4 with 768 everywhere, 98.2 and
+ * 96.8 with 1,400 and 4,096 for the heavy ones. */
+constexpr u32 LIGHT_BLOCKS = 768, HEAVY_BLOCKS = 2048;
+
+u32 parts_of(const Plan &g, u32 rows, u32 blocks) {
+    const u32 most = (g.steps + CWAVES - 1u) / CWAVES, want = rows < blocks ? blocks / rows : 1u; /* a wavefront has at least a step */
+    const u32 parts = want < most ? want : most;
+    return parts < MAX_CHUNKS ? parts : MAX_CHUNKS;
+}
 
 size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
     g.steps = (vocab + STEP - 1u) / STEP;
-    /* about 2,048 blocks (192 rows of 129,280 fp16: 94.9 us, with 1,024 103.1; blocks of 256 threads 99.2); a wavefront
-     * has at least a step */
-    const u32 most = (g.steps + CWAVES - 1u) / CWAVES, want = rows < 2048u ? 2048u / rows : 1u;
-    g.chunks = want < most ? want : most;
-    if (g.chunks > MAX_CHUNKS) g.chunks = MAX_CHUNKS;
-    g.run = (g.steps + g.chunks - 1u) / g.chunks;
+    g.chunks = parts_of(g, rows, LIGHT_BLOCKS);
     g.shift = shift_of(vocab);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -757,6 +954,7 @@ size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
         return (void *)p;
     };
     g.max_rank = (u64 *)take((size_t)rows * MAX_CHUNKS * 8u);
+    g.tops = (u32 *)take((size_t)rows * g.steps * 4u);
     g.weight = (u64 *)take((size_t)rows * BINS * 8u);
     g.count = (u32 *)take((size_t)rows * BINS * 4u);
     g.list = (u64 *)take((size_t)rows * LIST * 8u);
@@ -769,7 +967,7 @@ size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
 
 template <bool F32>
 hipError_t launch(hipStream_t st, const uocr_sample_args &a) {
-    if (a.vocab <= ONE_BLOCK) {
+    if (by_one_block(a.rows, a.vocab)) {
         hipLaunchKernelGGL((k_sample_row<F32>), dim3(a.rows), dim3(NT), 0, st, a, shift_of(a.vocab));
         return hipGetLastError();
     }
@@ -777,14 +975,18 @@ hipError_t launch(hipStream_t st, const uocr_sample_args &a) {
     g.a = a;
     (void)lay_out(g, a.rows, a.vocab, (uint8_t *)a.ws);
     g.cut = a.top_k != nullptr || a.top_p != nullptr;
-    const dim3 grid(a.rows * g.chunks), block(CT);
-    hipLaunchKernelGGL((k_sample_max<F32>), grid, block, 0, st, g);
+    auto go = [&](void (*kernel)(Plan), u32 blocks) {
+        g.parts = parts_of(g, a.rows, blocks);
+        g.run = (g.steps + g.parts - 1u) / g.parts;
+        hipLaunchKernelGGL(kernel, dim3(a.rows * g.parts), dim3(CT), 0, st, g);
+    };
+    go(k_sample_max<F32>, LIGHT_BLOCKS);
     if (g.cut) {
-        hipLaunchKernelGGL((k_sample_bins<F32>), grid, block, 0, st, g);
-        hipLaunchKernelGGL((k_sample_list<F32>), grid, block, 0, st, g);
+        go(k_sample_bins<F32>, HEAVY_BLOCKS);
+        go(k_sample_list<F32>, LIGHT_BLOCKS);
         hipLaunchKernelGGL((k_sample_cut<F32>), dim3(a.rows), dim3(LIST), 0, st, g);
     }
-    hipLaunchKernelGGL((k_sample_sums<F32>), grid, block, 0, st, g);
+    go(k_sample_sums<F32>, HEAVY_BLOCKS);
     hipLaunchKernelGGL((k_sample_pick<F32>), dim3(a.rows), dim3(NT), 0, st, g);
     return hipGetLastError();
 }
@@ -792,7 +994,7 @@ hipError_t launch(hipStream_t st, const uocr_sample_args &a) {
 }  // namespace
 
 size_t uocr_sample_ws_bytes(uint32_t rows, uint32_t vocab) {
-    if (vocab <= ONE_BLOCK || rows == 0u) return 16u;
+    if (rows == 0u || by_one_block(rows, vocab)) return 16u;
     Plan g;
     return lay_out(g, rows, vocab, nullptr);
 }
