@@ -307,7 +307,11 @@ UOCR_API int uocr_op_moe_ffn_rows_static(const uocr_op_moe_weights *m, const voi
  * by the kernels, as said at each, so a bad value never leads out of range.
  * Device pointers belong to device 0; operands that another stream writes have
  * to be finished first.  All of them can be captured (uocr_hip_capture_begin),
- * with no allocation inside; a replay reads the device-side values anew. */
+ * with no allocation inside; a replay reads the device-side values anew.
+ * Limits beside those said below: 1,024 heads, 65,536 sequences or rows of
+ * logits, 8,388,607 tokens of kv_append and kv_gather, as much for n_seqs *
+ * heads of uocr_op_paged_attention and for (q_tokens / 64 + n_seqs) * heads of
+ * uocr_op_packed_attention; scale up to 2^64. */
 
 /* A paged KV cache.  Token p of sequence s stands in page
  * page_table[s * table_stride + p / page_tokens], at slot p % page_tokens of
@@ -334,8 +338,8 @@ typedef struct uocr_op_kv_pages {
 
 /* Writes the keys and values of `tokens` new tokens into their pages and
  * rotates queries and keys to their positions (split-half RoPE over the whole
- * head, angle = position * rope_theta^(-2 i / head_dim), exact to 2^-25 turns
- * for every int32 position; rope_theta 0: no rotation).  Token i belongs to
+ * head, angle = position * rope_theta^(-2 i / head_dim), formed in fp64 and
+ * off by 2^-23 turns at most; rope_theta from 1, or 0: no rotation).  Token i belongs to
  * sequence seqs[i] (NULL: sequence i) at positions[i].  Rows are
  * [heads][head_dim] fp16 (k, v: [kv_heads][head_dim]), q_stride .. v_stride
  * values from one token to the next (at least a row).  q NULL: no queries;
@@ -374,8 +378,10 @@ UOCR_API size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_
  * h / (heads / kv_heads).  q and out fp16 [n_seqs][heads][head_dim], strides in
  * values from one sequence to the next (out may be q); scale 0: 1 /
  * sqrt(head_dim).  fp32 softmax and sums; probabilities (Q8_0: times the
- * values' scales) enter the products in fp16.  Tokens in absent pages are left out; where none is
- * left the row is zero.  Beside uocr_op_attention_decode. */
+ * values' scales) enter the products in fp16, where one below 2^-25 is zero
+ * (and NaN beside a value that is not finite).  Tokens in absent pages are
+ * left out; where none is left the row is zero.  Beside
+ * uocr_op_attention_decode. */
 UOCR_API int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_t *lengths, uint32_t heads, float scale,
                                      const void *q, uint64_t q_stride, void *workspace, void *out,
                                      uint64_t out_stride);
@@ -390,16 +396,17 @@ UOCR_API int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int32_
  * fp16 [q_tokens][heads][head_dim], k and v [k_tokens][kv_heads][head_dim],
  * strides in values from one token to the next (below 2^22); query head h
  * takes KV head h / (heads / kv_heads); head_dim 64 or 128; scale 0: 1 /
- * sqrt(head_dim).  fp32 softmax and sums, fp16 probabilities.  Values that a
- * row does not see never reach it, not finite ones either.  Beside
- * uocr_op_prefill_attention. */
+ * sqrt(head_dim); out may be q.  fp32 softmax and sums, fp16 probabilities.
+ * Values that a row does not see never reach it, not finite ones either.
+ * Beside uocr_op_prefill_attention. */
 UOCR_API int uocr_op_packed_attention(uint32_t n_seqs, const int32_t *q_starts, uint32_t q_tokens,
                                       const int32_t *k_starts, uint32_t k_tokens, uint32_t heads, uint32_t kv_heads,
                                       uint32_t head_dim, float scale, const void *q, uint64_t q_stride, const void *k,
                                       uint64_t k_stride, const void *v, uint64_t v_stride, void *out,
                                       uint64_t out_stride);
 
-/* Bytes of uocr_op_sample's workspace (any contents). */
+/* Bytes of uocr_op_sample's workspace (any contents), or 0 for sizes that it
+ * refuses. */
 UOCR_API size_t uocr_op_sample_workspace_bytes(uint32_t rows, uint32_t vocab);
 
 /* A token of each row of logits ([rows][vocab], `stride` values apart; type 1

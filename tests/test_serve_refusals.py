@@ -56,12 +56,13 @@ APPEND = dict(tokens=2, seqs=None, pos=AT, heads=2, theta=1e4, q=AT, qs=128, q_o
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(pos=None), "positions"), (dict(pos=AT + 1), "positions"), (dict(seqs=AT + 2), "positions"), (dict(tokens=3), "a sequence for each token"),
-    (dict(tokens=1 << 31, seqs=AT), "positions"), (dict(heads=0), "q and q_out"), (dict(heads=2000), "q and q_out"), (dict(q_out=None), "q and q_out"),
+    (dict(pos=None), "positions"), (dict(pos=AT + 1), "positions"), (dict(seqs=AT + 2), "positions"), (dict(tokens=3), "a sequence for each"),
+    (dict(tokens=1 << 31, seqs=AT), "positions"), (dict(tokens=1 << 23, seqs=AT), "positions"), (dict(heads=0), "q and q_out"), (dict(heads=2000), "q and q_out"), (dict(q_out=None), "q and q_out"),
     (dict(q=None), "q and q_out"), (dict(qs=127), "q and q_out"), (dict(qos=64), "q and q_out"), (dict(q=AT + 1), "q and q_out"),
     (dict(q_out=AT, qos=256), "q and q_out"), (dict(k=None), "k and v rows"), (dict(ks=100), "k and v rows"), (dict(v=None), "k and v rows"),
     (dict(vs=0), "k and v rows"), (dict(k_out=AT, kos=64), "k and v rows"), (dict(k_out=AT, kos=256), "k and v rows"),
     (dict(v=AT + 1), "k and v rows"), (dict(theta=-1.0), "rope_theta"), (dict(theta=float("nan")), "rope_theta"), (dict(theta=float("inf")), "rope_theta"),
+    (dict(theta=0.5), "rope_theta"),
 ], ids=str)
 def test_append_refusals(uocr, change, match):
     a = {**APPEND, **change}
@@ -69,7 +70,7 @@ def test_append_refusals(uocr, change, match):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(pos=None), "positions"), (dict(seqs=AT + 1), "positions"), (dict(tokens=3), "a sequence for each token"), (dict(k=None, v=None), "k_out or v_out"),
+    (dict(pos=None), "positions"), (dict(seqs=AT + 1), "positions"), (dict(tokens=3), "a sequence for each"), (dict(tokens=1 << 23, seqs=AT), "positions"), (dict(k=None, v=None), "k_out or v_out"),
     (dict(ks=127), "k_out or v_out"), (dict(vs=127), "k_out or v_out"), (dict(v=AT + 1), "k_out or v_out"),
 ], ids=str)
 def test_gather_refusals(uocr, change, match):
@@ -79,7 +80,7 @@ def test_gather_refusals(uocr, change, match):
 
 @pytest.mark.parametrize("change,match", [
     (dict(lengths=None), "lengths"), (dict(lengths=AT + 2), "lengths"), (dict(heads=0), "multiple of kv_heads"), (dict(heads=3), "multiple of kv_heads"),
-    (dict(heads=2048), "multiple of kv_heads"), (dict(scale=-1.0), "a scale"), (dict(scale=float("nan")), "a scale"), (dict(scale=float("inf")), "a scale"),
+    (dict(heads=2048), "multiple of kv_heads"), (dict(scale=-1.0), "a scale"), (dict(scale=float("nan")), "a scale"), (dict(scale=float("inf")), "a scale"), (dict(scale=1e20), "a scale"),
     (dict(q=None), "lengths"), (dict(qs=255), "lengths"), (dict(ws=None), "workspace"), (dict(ws=AT + 8), "workspace"), (dict(out=None), "lengths"),
     (dict(os=255), "lengths"), (dict(out=AT + 1), "lengths"), (dict(q=AT, out=AT, os=512), "lengths"),
 ], ids=str)
@@ -93,7 +94,7 @@ def test_paged_refusals(uocr, change, match):
     (dict(qt=1 << 31), "tokens"), (dict(kt=1 << 31), "tokens"), (dict(kst=None, kt=9), "as many keys"), (dict(heads=0), "head_dim"), (dict(heads=5), "head_dim"),
     (dict(heads=2048), "head_dim"), (dict(kvh=0), "head_dim"), (dict(dim=80), "head_dim"), (dict(scale=-0.5), "head_dim"), (dict(scale=float("nan")), "head_dim"),
     (dict(q=None), "q and out"), (dict(qs=255), "q and out"), (dict(out=None), "q and out"), (dict(os=0), "q and out"), (dict(q=AT + 1), "q and out"),
-    (dict(out=AT, os=512), "q and out"), (dict(k=None), "k and v"), (dict(v=None), "k and v"), (dict(ks=127), "k and v"), (dict(vs=1 << 22), "k and v"),
+    (dict(out=AT, os=512), "q and out"), (dict(qt=1 << 30), "(q_tokens / 64"), (dict(n=1 << 16, heads=512), "(q_tokens / 64"), (dict(k=None), "k and v"), (dict(v=None), "k and v"), (dict(ks=127), "k and v"), (dict(vs=1 << 22), "k and v"),
 ], ids=str)
 def test_packed_refusals(uocr, change, match):
     a = {**dict(n=2, qst=AT, qt=8, kst=AT, kt=8, heads=4, kvh=2, dim=64, scale=0.0, q=AT, qs=256, k=AT, ks=128, v=AT, vs=128, out=AT, os=256), **change}
@@ -112,8 +113,17 @@ def test_sample_refusals(uocr, change, match):
     refused(uocr, "uocr_op_sample", *a.values(), match=match)
 
 
+def test_paged_too_many_rows(uocr):
+    c = ct.byref(cache(uocr, n_seqs=1 << 16))
+    refused(uocr, "uocr_op_paged_attention", c, AT, 128, 0.0, AT, 1 << 13, AT, AT, 1 << 13, match="n_seqs * heads")
+
+
 def test_workspace_sizes(uocr):
     assert uocr.paged_attention_workspace_bytes(4, 10, 10, 128) > 0
     for bad in ((0, 4, 2, 64), (1, 0, 1, 64), (1, 5, 2, 64), (1, 4, 0, 64), (1, 4, 2, 80), (1 << 20, 4, 2, 64)):
         assert uocr.paged_attention_workspace_bytes(*bad) == 0
+    assert uocr.paged_attention_workspace_bytes(1 << 16, 128, 2, 64) == 0
     assert uocr.sample_workspace_bytes(1, 129280) > 0
+    assert uocr.sample_workspace_bytes(1 << 16, 1 << 24) > 0
+    for bad in ((1, 0), (1, (1 << 24) + 1), (1, 0xffffffff), ((1 << 16) + 1, 100)):
+        assert uocr.sample_workspace_bytes(*bad) == 0

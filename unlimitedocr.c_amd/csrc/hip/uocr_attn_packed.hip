@@ -338,11 +338,10 @@ hipError_t launch(hipStream_t st, const uocr_packed_args &a) {
     g.slots = a.q_tokens / (WQ * 32u) + a.n_seqs;
     g.group = a.heads / a.kv_heads;
     g.c = a.scale * 1.4426950408889634f;
-    const uint64_t blocks = (uint64_t)g.slots * a.heads;
-    if (blocks > 0x7fffffffu) return hipErrorInvalidValue;
+    const u32 blocks = g.slots * a.heads; /* the operator's limit keeps it in range */
     const bool dma = ((((uintptr_t)a.k | (uintptr_t)a.v) & 15u) | ((a.ks | a.vs) & 7u)) == 0u;
-    if (dma) hipLaunchKernelGGL((k_packed_attention<D, WQ, WG, KT, NB, true>), dim3((u32)blocks), dim3(64 * WQ * WG), 0, st, g);
-    else hipLaunchKernelGGL((k_packed_attention<D, WQ, WG, KT, NB, false>), dim3((u32)blocks), dim3(64 * WQ * WG), 0, st, g);
+    if (dma) hipLaunchKernelGGL((k_packed_attention<D, WQ, WG, KT, NB, true>), dim3(blocks), dim3(64 * WQ * WG), 0, st, g);
+    else hipLaunchKernelGGL((k_packed_attention<D, WQ, WG, KT, NB, false>), dim3(blocks), dim3(64 * WQ * WG), 0, st, g);
     return hipGetLastError();
 }
 

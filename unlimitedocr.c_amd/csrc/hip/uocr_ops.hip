@@ -691,7 +691,7 @@ bool rows_ok(const void *p, uint64_t stride, uint64_t heads, uint64_t dim) {
 }
 
 bool scale_ok(float scale) {
-    return scale >= 0.0f && scale <= 1.8446744e19f; /* false for NaN; scores stay finite in fp32 */
+    return scale >= 0.0f && scale <= 0x1p64f; /* false for NaN; scores stay finite in fp32 */
 }
 
 }  // namespace
@@ -706,9 +706,9 @@ extern "C" int uocr_op_kv_append(const uocr_op_kv_pages *pages, uint32_t tokens,
     const int r = pages_of(pages, "kv_append", &a.kv);
     if (r != UOCR_OK) return r;
     const uint32_t kvh = a.kv.heads, dim = a.kv.dim;
-    if (tokens > 0x7fffffffu || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
+    if (tokens > UOCR_SERVE_MAX_TOKENS || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
         (seqs == nullptr && tokens > a.kv.n_seqs)) {
-        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: positions, and a sequence for each token, are needed");
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: positions, and a sequence for each of up to %u tokens, are needed", UOCR_SERVE_MAX_TOKENS);
     }
     if (q != nullptr ? heads == 0u || heads > UOCR_SERVE_MAX_HEADS || !rows_ok(q, q_stride, heads, dim) ||
                            !rows_ok(q_out, q_out_stride, heads, dim) || (q_out == q && q_out_stride != q_stride)
@@ -720,8 +720,8 @@ extern "C" int uocr_op_kv_append(const uocr_op_kv_pages *pages, uint32_t tokens,
         (k_out != nullptr && (!rows_ok(k_out, k_out_stride, kvh, dim) || (k_out == k && k_out_stride != k_stride)))) {
         return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: k and v rows are at least kv_heads * head_dim apart");
     }
-    if (!(rope_theta >= 0.0f && rope_theta <= 3.0e38f)) {
-        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: rope_theta is positive, or 0 for no rotation");
+    if (!(rope_theta == 0.0f || (rope_theta >= 1.0f && rope_theta <= 3.0e38f))) { /* below 1 the angles outgrow fp64 */
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_append: rope_theta is 1 or more, or 0 for no rotation");
     }
     STREAM_OR_RETURN(st);
     if (tokens == 0u) return UOCR_OK;
@@ -752,9 +752,9 @@ extern "C" int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens,
     memset(&a, 0, sizeof(a));
     const int r = pages_of(pages, "kv_gather", &a.kv);
     if (r != UOCR_OK) return r;
-    if (tokens > 0x7fffffffu || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
+    if (tokens > UOCR_SERVE_MAX_TOKENS || positions == nullptr || off(positions, 4) || (seqs != nullptr && off(seqs, 4)) ||
         (seqs == nullptr && tokens > a.kv.n_seqs)) {
-        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_gather: positions, and a sequence for each token, are needed");
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "kv_gather: positions, and a sequence for each of up to %u tokens, are needed", UOCR_SERVE_MAX_TOKENS);
     }
     if ((k_out == nullptr && v_out == nullptr) ||
         (k_out != nullptr && !rows_ok(k_out, k_out_stride, a.kv.heads, a.kv.dim)) ||
@@ -777,7 +777,7 @@ extern "C" int uocr_op_kv_gather(const uocr_op_kv_pages *pages, uint32_t tokens,
 extern "C" size_t uocr_op_paged_attention_workspace_bytes(uint32_t n_seqs, uint32_t heads, uint32_t kv_heads,
                                                           uint32_t head_dim) {
     if (n_seqs == 0u || n_seqs > UOCR_SERVE_MAX_SEQS || kv_heads == 0u || heads == 0u || heads > UOCR_SERVE_MAX_HEADS ||
-        heads % kv_heads != 0u || (head_dim != 64u && head_dim != 128u)) {
+        heads % kv_heads != 0u || (head_dim != 64u && head_dim != 128u) || (uint64_t)n_seqs * heads > UOCR_SERVE_MAX_TOKENS) {
         return 0u;
     }
     return uocr_paged_attention_ws_bytes(heads, kv_heads, head_dim);
@@ -790,14 +790,15 @@ extern "C" int uocr_op_paged_attention(const uocr_op_kv_pages *pages, const int3
     memset(&a, 0, sizeof(a));
     const int r = pages_of(pages, "paged_attention", &a.kv);
     if (r != UOCR_OK) return r;
-    if (heads == 0u || heads > UOCR_SERVE_MAX_HEADS || heads % a.kv.heads != 0u) {
-        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "paged_attention: heads is a multiple of kv_heads up to %u", UOCR_SERVE_MAX_HEADS);
+    if (heads == 0u || heads > UOCR_SERVE_MAX_HEADS || heads % a.kv.heads != 0u || (uint64_t)a.kv.n_seqs * heads > UOCR_SERVE_MAX_TOKENS) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "paged_attention: heads is a multiple of kv_heads up to %u, n_seqs * heads up to %u",
+                       UOCR_SERVE_MAX_HEADS, UOCR_SERVE_MAX_TOKENS);
     }
     if (lengths == nullptr || off(lengths, 4) || workspace == nullptr || off(workspace, 16) || !scale_ok(scale) ||
         !rows_ok(q, q_stride, heads, a.kv.dim) || !rows_ok(out, out_stride, heads, a.kv.dim) ||
         (out == q && out_stride != q_stride)) {
         return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
-                       "paged_attention: lengths, a workspace on 16 bytes, a scale from 0 and rows at least heads * head_dim apart are needed");
+                       "paged_attention: lengths, a workspace on 16 bytes, a scale from 0 to 2^64 and rows at least heads * head_dim apart are needed");
     }
     STREAM_OR_RETURN(st);
     const on_device0 dev;
@@ -826,7 +827,10 @@ extern "C" int uocr_op_packed_attention(uint32_t n_seqs, const int32_t *q_starts
     if ((head_dim != 64u && head_dim != 128u) || kv_heads == 0u || heads == 0u || heads > UOCR_SERVE_MAX_HEADS ||
         heads % kv_heads != 0u || !scale_ok(scale)) {
         return op_fail(UOCR_ERROR_INVALID_ARGUMENT,
-                       "packed_attention: head_dim 64 or 128, heads a multiple of kv_heads up to %u, scale from 0", UOCR_SERVE_MAX_HEADS);
+                       "packed_attention: head_dim 64 or 128, heads a multiple of kv_heads up to %u, scale 0 to 2^64", UOCR_SERVE_MAX_HEADS);
+    }
+    if (((uint64_t)q_tokens / 64u + n_seqs) * heads > UOCR_SERVE_MAX_TOKENS) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "packed_attention: (q_tokens / 64 + n_seqs) * heads is up to %u", UOCR_SERVE_MAX_TOKENS);
     }
     if (q_tokens != 0u && (!rows_ok(q, q_stride, heads, head_dim) || !rows_ok(out, out_stride, heads, head_dim) ||
                            (out == q && out_stride != q_stride))) {
@@ -862,6 +866,7 @@ extern "C" int uocr_op_packed_attention(uint32_t n_seqs, const int32_t *q_starts
 }
 
 extern "C" size_t uocr_op_sample_workspace_bytes(uint32_t rows, uint32_t vocab) {
+    if (vocab == 0u || vocab > (1u << 24) || rows > UOCR_SERVE_MAX_SEQS) return 0u;
     return uocr_sample_ws_bytes(rows, vocab);
 }
 

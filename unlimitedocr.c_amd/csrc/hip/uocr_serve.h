@@ -15,6 +15,7 @@
 
 #define UOCR_SERVE_MAX_SEQS 65536u /* keeps grids and counts of tiles well inside their types */
 #define UOCR_SERVE_MAX_HEADS 1024u
+#define UOCR_SERVE_MAX_TOKENS 8388607u /* blocks of a launch, of up to 512 threads each: below 2^32 threads */
 
 /* A paged cache: page_stride in values; pages of 2^shift tokens. */
 struct uocr_kv {
