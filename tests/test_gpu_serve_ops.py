@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from conftest import convert_q8, rand_f16
-from serve_reference import H16, H32, SUB16, Pages, packed, paged, rotated, sample, stored
+from serve_reference import H16, H32, SUB16, Pages, attend, packed, paged, rotated, sample, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -323,6 +323,57 @@ def test_paged_attention_in_place_and_repeated(gpu):
     near(first.view(np.float16).reshape(q.shape), ref, tol, "paged")
 
 
+def test_paged_attention_largest_pages(gpu):
+    """Pages of 65,536 tokens, the second one hardly begun."""
+    rng = np.random.default_rng(16)
+    for qtype, lengths in ((1, [65541, 3]), (3, [65537])):
+        paged_case(gpu, rng, qtype, 2, 1, 64, 65536, lengths)
+
+
+@pytest.mark.parametrize("qtype", [1, 3])
+def test_offsets_past_32_bits(gpu, qtype):
+    """Pages 2^31 values apart, rows of keys 2^22 - 64: appended, read back, read by both attentions."""
+    rng = np.random.default_rng(17)
+    heads, kvh, dim, page, n, far = 2, 1, 64, 512, 1100, 2 ** 31
+    size = 2 if qtype == 1 else 1
+    pages = gpu.DeviceBuffer((2 * far + 2 * page * dim) * size)  # v's pages stand behind k's
+    scales = gpu.DeviceBuffer((2 * far + 2 * page * dim) // 64 * 2) if qtype == 3 else None
+    table = dev(gpu, np.array([[2, 0, 1]], np.int32))
+    desc = gpu.CKvPages(qtype=qtype, kv_heads=kvh, head_dim=dim, page_tokens=page, n_pages=3, n_seqs=1, table_stride=3, page_stride=far, k=pages.ptr,
+                        v=pages.ptr + page * dim * size, k_scales=scales.ptr if scales else None, v_scales=scales.ptr + page * dim // 64 * 2 if scales else None,
+                        page_table=table.ptr)
+    rows = rand_f16(rng, (3, n, 1, dim))
+    q, k, v = (dev(gpu, x) for x in rows)
+    seqs, pos = dev(gpu, np.zeros(n, np.int32)), dev(gpu, np.arange(n, dtype=np.int32))
+    gpu.op_kv_append(desc, n, seqs, pos, 0, 0.0, None, 0, None, 0, k, dim, None, 0, v, dim)
+    near_k, near_v = gpu.DeviceBuffer(2 * n * dim), gpu.DeviceBuffer(2 * n * dim)
+    gpu.op_kv_gather(desc, n, seqs, pos, near_k, dim, near_v, dim)
+    gpu.sync()
+    kk, vv = (b.download(np.float16).reshape(n, 1, dim) for b in (near_k, near_v))
+    held = [x.astype(np.float64).reshape(n, dim) for x in rows[1:]]
+    if qtype == 3:
+        for i, (q8, sc) in enumerate(convert_q8(x.astype(np.float32).reshape(n, dim)) for x in rows[1:]):
+            held[i] = q8.astype(np.float64) * sc.astype(np.float64)
+    for got, want in zip((kk, vv), held):
+        assert np.array_equal(got.reshape(n, dim), want.astype(np.float16))
+    qq = rows[0, :2].reshape(1, 2, dim)
+    out, ws = gpu.DeviceBuffer(2 * 2 * dim), gpu.DeviceBuffer(gpu.paged_attention_workspace_bytes(1, heads, kvh, dim))
+    gpu.op_paged_attention(desc, dev(gpu, np.array([n], np.int32)), heads, 0.0, dev(gpu, qq), heads * dim, ws, out, heads * dim)
+    stride = 2 ** 22 - 64
+    if qtype == 1:  # 9 GB of rows: keys and values beside each other
+        wide = gpu.DeviceBuffer((n * stride) * 2)
+        gpu.op_kv_gather(desc, n, seqs, pos, wide, stride, wide.ptr + 2 * dim, stride)
+        packed_out = gpu.DeviceBuffer(2 * n * dim)
+        gpu.op_packed_attention(1, dev(gpu, np.array([0, n], np.int32)), n, None, n, 1, 1, dim, 0.0, q, dim, wide, stride, wide.ptr + 2 * dim, stride,
+                                packed_out, dim)
+        gpu.sync()
+        ref, tol = packed(rows[0], kk, vv, [0, n], [0, n], dim ** -0.5)
+        near(packed_out.download(np.float16).reshape(n, 1, dim), ref, tol, "packed")
+    gpu.sync()
+    ref, tol = attend(qq[0].astype(np.float64), held[0], held[1], np.ones((2, n), bool), dim ** -0.5, 8.0 if qtype == 3 else 1.0)
+    near(out.download(np.float16).reshape(2, dim), ref, tol, "paged")
+
+
 # ---- packed prompts --------------------------------------------------------------------
 
 def packed_case(uocr, rng, heads, kvh, dim, nq, nk=None, scale=0.0, lead_rows=0, tail_rows=0, gaps=(0, 0, 0, 0), shift=0, change=None):
@@ -413,6 +464,21 @@ def test_packed_attention_values_that_are_not_finite(gpu, dim, heads, n):
         v[n - 1, 0, :], k[n, 0, :], v[n, 0, :] = np.nan, np.nan, np.inf
 
     packed_case(gpu, rng, heads, 1, dim, [n, 50], change=change)
+
+
+def test_packed_attention_in_place(gpu):
+    """out may be q, a value that is not finite among the rows that others do not see too."""
+    rng = np.random.default_rng(18)
+    nq, heads, kvh, dim = [300, 70], 6, 2, 128
+    starts = np.concatenate([[0], np.cumsum(nq)])
+    q, k, v = (rand_f16(rng, (370, h, dim)) for h in (heads, kvh, kvh))
+    v[299, 1, 7] = np.inf
+    d = [dev(gpu, x) for x in (q, k, v)]
+    gpu.op_packed_attention(2, dev(gpu, starts.astype(np.int32)), 370, None, 370, heads, kvh, dim, 0.0, d[0], heads * dim, d[1], kvh * dim, d[2], kvh * dim,
+                            d[0], heads * dim)
+    gpu.sync()
+    ref, tol = packed(q, k, v, starts, starts, dim ** -0.5)
+    near(d[0].download(np.float16).reshape(q.shape), ref, tol, "packed")
 
 
 def test_packed_attention_bad_starts(gpu):
@@ -660,3 +726,65 @@ def test_prompts_then_decode(gpu):
     assert np.array_equal(eager[0], graph[0]) and np.array_equal(eager[1], graph[1])
     for side in range(2):
         assert np.array_equal(c1.download().data[side].view(np.uint16), c2.download().data[side].view(np.uint16))
+
+
+def test_replays_of_every_operator(gpu):
+    """One graph with all operators (paged attention with both ways of joining, sampling in one block and in several) on shared
+    workspaces, replayed with other contents of its arrays, eager calls and synchronizations in between: the eager results' bits."""
+    rng = np.random.default_rng(33)
+    dim, page, n = 64, 16, 3
+    lengths = [700, 33, 1200]
+    sizes = [(32, 2), (8, 4)]  # joined by a launch of its own, and by the last block
+    caches = [Pages(rng, t, kvh, dim, page, [x + 8 for x in lengths]) for t, (_, kvh) in zip((1, 3), sizes)]
+    for c in caches:
+        c.fill(rng, lengths)
+    ws = gpu.DeviceBuffer(max(gpu.paged_attention_workspace_bytes(n, h, kvh, dim) for h, kvh in sizes))
+    vocabs = [900, 40000]
+    sws = gpu.DeviceBuffer(max(gpu.sample_workspace_bytes(n, x) for x in vocabs))
+    x = {name: gpu.DeviceBuffer(size) for name, size in dict(q=2 * n * 32 * dim, k=2 * n * 4 * dim, v=2 * n * 4 * dim, pos=4 * n, len=4 * n, starts=4 * (n + 1),
+                                                             logits=4 * n * vocabs[1], u=4 * n, top_p=4 * n, top_k=4 * n).items()}
+
+    def fresh(i):
+        r = np.random.default_rng(100 + i)
+        for name in ("q", "k", "v"):
+            x[name].upload(rand_f16(r, x[name].nbytes // 2))
+        pos = np.array(lengths, np.int32) + i
+        x["pos"].upload(pos)
+        x["len"].upload(pos + 1)
+        x["starts"].upload(np.array([0, i % 3, 2, 3], np.int32))
+        x["logits"].upload((r.standard_normal(n * vocabs[1]) * 3).astype(np.float32))
+        x["u"].upload(r.uniform(0, 1, n).astype(np.float32))
+        x["top_p"].upload(np.array([0.9, 1.0, 0.5], np.float32))
+        x["top_k"].upload(np.array([0, 40, 600], np.int32))
+
+    def outputs():
+        return [gpu.DeviceBuffer(size) for size in [2 * n * 32 * dim] * 4 + [2 * n * 4 * dim] * 4 + [4 * n] * 4]
+
+    def run(descs, o):
+        for i, ((h, kvh), desc) in enumerate(zip(sizes, descs)):
+            gpu.op_kv_append(desc, n, None, x["pos"], h, 1e4, x["q"], h * dim, o[i], h * dim, x["k"], kvh * dim, None, 0, x["v"], kvh * dim)
+            gpu.op_paged_attention(desc, x["len"], h, 0.0, o[i], h * dim, ws, o[2 + i], h * dim)
+            gpu.op_kv_gather(desc, n, None, x["pos"], o[4 + 2 * i], kvh * dim, o[5 + 2 * i], kvh * dim)
+            gpu.op_packed_attention(n, x["starts"], n, None, n, h, kvh, dim, 0.0, o[i], h * dim, o[4 + 2 * i], kvh * dim, o[5 + 2 * i], kvh * dim, o[i], h * dim)
+            gpu.op_sample(gpu.QT_F32, n, vocabs[i], x["logits"], vocabs[i], None, x["top_k"], x["top_p"], None, x["u"], sws, o[8 + 2 * i], o[9 + 2 * i])
+
+    eager, held = outputs(), outputs()
+    d1 = [c.upload(gpu) for c in caches]
+    keep = [(c.dev, c.dev_s, c.dev_t) for c in caches]
+    d2 = [c.upload(gpu) for c in caches]
+    fresh(0)
+    run(d1, eager)
+    gpu.sync()
+    with gpu.Capture() as cap:
+        run(d2, held)
+    for i in range(6):
+        fresh(i)
+        run(d1, eager)
+        if i % 2:
+            gpu.sync()
+        cap.replay(1)
+        gpu.sync()
+        for j, (a, b) in enumerate(zip(eager, held)):
+            assert np.array_equal(a.download(np.uint16), b.download(np.uint16)), f"replay {i}, output {j}"
+    cap.release()
+    assert len(keep) == 2
