@@ -610,7 +610,7 @@ def test_sample_long_crowded_rows(gpu, f32):
         sample_case(gpu, x, f32, u=u, **s)
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 16384), (1, 16385), (64, 32768), (64, 32769), (63, 20000), (2, 300007), (1, 1500000)])
+@pytest.mark.parametrize("rows,vocab", [(1, 16384), (1, 16385), (64, 32768), (64, 32769), (63, 20000), (128, 32768), (128, 32769), (2, 300007), (1, 1500000)])
 def test_sample_one_block_or_several(gpu, rows, vocab):
     """Sizes on both sides of where rows are shared, rows of more than 512 steps, each row with settings of its own."""
     rng = np.random.default_rng(rows + vocab)

@@ -1,11 +1,9 @@
 /*
  * uocr_sample.hip - sampling a token of each row of logits on gfx950.
  */
+#include "uocr_dev.h"
 #include "uocr_serve.h"
 
-#include <math.h>
-
-typedef uint32_t u32;
 typedef unsigned long long u64;
 
 namespace {
@@ -14,13 +12,17 @@ constexpr u32 NT = 1024, WAVES = NT / 64; /* a block that has a row of its own *
 constexpr u32 CT = 512, CWAVES = CT / 64; /* a block that has a part of a row */
 constexpr u32 ROW_U = 1;                  /* steps that it loads at a time: its registers hold no more */
 constexpr u32 E = 8, STEP = 64 * E;       /* values of a lane and of a wavefront per step */
+constexpr u32 ILP = 4;                     /* of them that are weighed side by side */
 constexpr u32 BINS = 2048;
 constexpr u32 LIST = 1024;                /* values that are ordered at once, one a thread */
 constexpr u32 GROUPS = 64;                /* partial sums of a wavefront's run in the last pass */
 constexpr u32 IDX_BITS = 24, IDX_MASK = (1u << IDX_BITS) - 1u;
-constexpr u32 TAB = 1024;                 /* 2^(i / TAB) */
+constexpr u32 TAB = 64;                   /* 2^(i / TAB): 64 doubles, two to a pair of LDS banks */
 constexpr u32 MAX_CHUNKS = 64;
 constexpr u32 TOPS = 512;                 /* groups of steps whose largest logits bound top-k */
+constexpr u32 FEW = 128;                  /* values that are all counted against each other */
+constexpr u32 COUNTED = 512;              /* bins whose values are counted for top-p alone: weights from e^-8 on */
+constexpr u64 DONE = ~0ull;               /* instead of a rank: the row has its token */
 
 /* Weights are integers in units of 2^-shift, shift = 62 - log2(vocab) rounded
  * up (50 at most): their sums neither overflow nor depend on the order of
@@ -36,6 +38,7 @@ struct Row {
     u32 shift, k;
     float p;
     bool inf, use_k, use_p;
+    bool hot;      /* a temperature above 0 */
 };
 
 /* Order-preserving key of a logit; NaN as -inf, -0 as 0. */
@@ -54,16 +57,17 @@ __device__ __forceinline__ u64 rank_of(float x, u32 id) {
 }
 
 /* A weight in units, not yet rounded: 2^shift exp((x - top) / temperature), as
- * 2^(n / TAB) from the table, a third-degree sum for the rest of |r| <= 1/2
- * (off by 2^-50) and the exponent.  fp64: next to a limit the last bits decide
- * which token it is, and fp64 runs at the rate of fp32 here. */
+ * 2^(n / TAB) from the table, a fifth-degree sum for the rest, f <= 1/2 (off
+ * by 2^-54), and the exponent (never below -986).  fp64: next to a limit the last bits decide which
+ * token it is. */
 __device__ __forceinline__ double weight(const Row &r, const double *tab, float x) {
     constexpr double L = 0.6931471805599453 / TAB;
     const double y = fmax(((double)x - (double)r.top) * r.c, -65536.0); /* NaN, too: no weight */
     const double big = y + 6755399441055744.0, f = y - (big - 6755399441055744.0);
     const int n = (int)(u32)__double_as_longlong(big);
-    const double p = fma(fma(fma(L * L * L / 6.0, f, L * L / 2.0), f, L), f, 1.0);
-    return ldexp(tab[(u32)n & (TAB - 1u)] * p, (n >> 10) + (int)r.shift);
+    const double p = fma(fma(fma(fma(fma(L * L * L * L * L / 120.0, f, L * L * L * L / 24.0), f, L * L * L / 6.0), f, L * L / 2.0), f, L), f, 1.0);
+    const u64 w = (u64)__double_as_longlong(tab[(u32)n & (TAB - 1u)] * p);
+    return __longlong_as_double((long long)(w + ((u64)(u32)((n >> 6) << 20) << 32)));
 }
 __device__ __forceinline__ u64 units(double w) {
     return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
@@ -85,8 +89,9 @@ constexpr Powers powers() {
 }
 __device__ const Powers g_powers = powers();
 
-__device__ __forceinline__ void fill_table(double *tab) {
-    for (u32 i = threadIdx.x; i < TAB; i += blockDim.x) tab[i] = g_powers.v[i];
+/* In units. */
+__device__ __forceinline__ void fill_table(double *tab, u32 shift) {
+    if (threadIdx.x < TAB) tab[threadIdx.x] = ldexp(g_powers.v[threadIdx.x], (int)shift);
 }
 
 /* Bins of equal width below the largest logit, over the range where a weight
@@ -95,27 +100,36 @@ __device__ __forceinline__ u32 bin_of(const Row &r, float x) {
     return x == r.top ? 0u : (u32)fminf((r.top - x) * r.scale, (float)(BINS - 1u)); /* NaN: the last */
 }
 
-/* The settings of row b whose largest logit has rank max_rank.  With a +inf
- * one, logits are taken as 0 there and -inf elsewhere (value_of). */
-__device__ __forceinline__ Row row_of(const uocr_sample_args &a, u32 b, u64 max_rank, float temp, u32 shift) {
+/* The settings of row b; cut: the distance from the largest logit. */
+__device__ __forceinline__ Row settings_of(const uocr_sample_args &a, u32 b, u32 shift) {
     Row r;
-    r.top = of_key((u32)(max_rank >> IDX_BITS));
-    r.inf = r.top == INFINITY;
-    if (r.inf) r.top = 0.0f;
+    const float temp = a.temperature != nullptr ? a.temperature[b] : 1.0f;
+    r.hot = temp > 0.0f;
+    r.top = 0.0f;
+    r.inf = false;
     r.shift = shift;
     r.c = (double)TAB * 1.4426950408889634 / (double)temp;
     r.scale = (float)((double)(BINS - 1u) / TAB * r.c / (double)(shift + 1u));
     const float m = a.min_p != nullptr && a.min_p[b] > 0.0f ? fminf(a.min_p[b], 1.0f) : 0.0f;
     r.min_w = ldexp((double)m, (int)shift);
-    /* below: lighter than min_p by more than the roundings here (2^-20 of the distance, and of the logit) */
-    const float far = temp * logf(m); /* -inf without min_p */
-    r.cut = r.top + far - 1e-6f * (fabsf(r.top) + fabsf(far));
-    if (!(r.cut > -INFINITY)) r.cut = -INFINITY;
+    r.cut = temp * logf(m); /* -inf without min_p */
     r.k = a.top_k != nullptr && a.top_k[b] > 0 ? (u32)a.top_k[b] : 0u;
     r.p = a.top_p != nullptr ? a.top_p[b] : 1.0f;
     r.use_k = r.k != 0u && r.k < a.vocab;
     r.use_p = r.p < 1.0f;
     return r;
+}
+
+/* With the rank of the row's largest logit.  Where that is +inf, logits are
+ * taken as 0 there and -inf elsewhere (value_of). */
+__device__ __forceinline__ void set_top(Row &r, u64 max_rank) {
+    r.top = of_key((u32)(max_rank >> IDX_BITS));
+    r.inf = r.top == INFINITY;
+    if (r.inf) r.top = 0.0f;
+    /* below: lighter than min_p by more than the roundings here (2^-20 of the distance, and of the logit) */
+    const float far = r.cut;
+    r.cut = r.top + far - 1e-6f * (fabsf(r.top) + fabsf(far));
+    if (!(r.cut > -INFINITY)) r.cut = -INFINITY;
 }
 
 /* The E values of the lane at id0; NaN, which takes part in nothing, outside the row. */
@@ -185,9 +199,7 @@ __device__ __forceinline__ float step_largest(u32 s, const float *x, float &best
 #pragma unroll
         for (int e = E - 1; e >= 0; --e) best_id = x[e] == m ? id0 + e : best_id;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    return m;
+    return wave_max_dpp(m);
 }
 
 __device__ __forceinline__ float value_of(const Row &r, float x) {
@@ -200,27 +212,44 @@ __device__ __forceinline__ void row_values(const void *row, u32 vocab, float lea
     each_step<F32, ROW_U>(row, vocab, threadIdx.x >> 6, (vocab + STEP - 1u) / STEP, WAVES, [&](u32 s, const float *x) { values_from(least, s, x, f); });
 }
 
-__device__ __forceinline__ u64 shfl64(u64 v, int src) {
-    return ((u64)(u32)__shfl((int)(v >> 32), src) << 32) | (u32)__shfl((int)v, src);
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    return ((u64)(u32)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (u32)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <int CTRL>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+    return ((u64)(u32)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true) << 32) |
+           (u32)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int m) {
     return ((u64)(u32)__shfl_xor((int)(v >> 32), m) << 32) | (u32)__shfl_xor((int)v, m);
 }
+/* Sum and maximum of all lanes (all of them active), as wave_sum. */
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
-    return v;
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    v += dpp64<0x140>(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+    v = max(v, dpp64<0xB1>(v));
+    v = max(v, dpp64<0x4E>(v));
+    v = max(v, dpp64<0x141>(v));
+    v = max(v, dpp64<0x140>(v));
+    return max(max(lane64(v, 0), lane64(v, 16)), max(lane64(v, 32), lane64(v, 48)));
 }
 
-/* Sums of what earlier lanes hold. */
+/* Sums of what earlier lanes hold: row_shr by 1, 2, 4, 8 within 16 lanes (zeros
+ * come in), then the rows'. */
 __device__ __forceinline__ u64 wave_before(u64 v) {
     u64 s = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl64(s, (int)(threadIdx.x & 63u) - d);
-        if ((int)(threadIdx.x & 63u) >= d) s += o;
-    }
-    return s - v;
+    s += dpp64<0x111>(s);
+    s += dpp64<0x112>(s);
+    s += dpp64<0x114>(s);
+    s += dpp64<0x118>(s);
+    const u64 a = lane64(s, 15), b = a + lane64(s, 31), c = b + lane64(s, 47);
+    const u32 row = (threadIdx.x & 63u) >> 4;
+    return s - v + (row == 0u ? 0ull : row == 1u ? a : row == 2u ? b : c);
 }
 
 struct Shared {
@@ -228,7 +257,7 @@ struct Shared {
     u64 weight[BINS];
     u32 count[BINS];
     u64 list[LIST];
-    u32 tops[TOPS], place[512];
+    u32 tops[TOPS], place[LIST], start[LIST];
     u64 red[WAVES];
     u64 red2[WAVES];
     u64 out[4];
@@ -250,16 +279,16 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *red, u64 &all) {
     return before;
 }
 
-/* The ranks of the block's LIST threads, largest first; the first n threads have
- * one, the others 0.  Few are counted against each other, by all threads (256:
- * 1 us); from about 400 on a bitonic sort, by lane exchange within wavefronts,
- * is the faster one (7 us). */
-__device__ __forceinline__ u64 sorted(u64 rank, u32 n, u64 *buf, u32 *place) {
-    const u32 t = threadIdx.x;
-    u32 size = 64u;
-    while (size < n) size <<= 1;
-    if (n <= 384u) {
-        const u32 parts = LIST / size, part = t / size, e = t % size;
+/* The ranks of the first n threads, largest first.  Few are counted against each
+ * other, by all threads.  More go to LIST buckets of equal width first, and are
+ * counted within them (equal logits share a bucket, at worst all of them): the
+ * launch of 192 rows' lists took 14.8 us with a bitonic sort, 11.1 so. */
+__device__ __forceinline__ u64 sorted(u64 rank, u32 n, Shared &sm) {
+    const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+    u64 *buf = sm.list;
+    u32 *place = sm.place;
+    if (n <= FEW) {
+        const u32 size = n <= 64u ? 64u : FEW, parts = LIST / size, part = t / size, e = t % size;
         if (t < size) {
             buf[t] = rank;
             place[t] = 0u;
@@ -275,27 +304,39 @@ __device__ __forceinline__ u64 sorted(u64 rank, u32 n, u64 *buf, u32 *place) {
         }
         __syncthreads();
         if (t < n) buf[place[t]] = rank;
+    } else {
+        const float x = of_key((u32)(rank >> IDX_BITS));
+        const bool in = t < n, finite = in && x > -INFINITY;
+        const float hi = wave_max_dpp(finite ? x : -INFINITY), lo = -wave_max_dpp(finite ? -x : -INFINITY);
+        float *ends = (float *)sm.red; /* [WAVES][2] */
+        if (lane == 0u) ends[2u * wave] = hi, ends[2u * wave + 1u] = -lo;
+        place[t] = 0u;
         __syncthreads();
-        rank = t < n ? buf[t] : 0ull;
+        const float end = wave_max_dpp(lane < 2u * WAVES && lane % 2u == 0u ? ends[lane] : -INFINITY);
+        const float low = -wave_max_dpp(lane < 2u * WAVES && lane % 2u == 1u ? ends[lane] : -INFINITY);
+        const float scale = end > low ? ((float)LIST - 0.5f) / (end - low) : 0.0f;
+        const u32 bucket = x == end ? 0u : (u32)fminf((end - x) * scale, (float)(LIST - 1u)); /* -inf: the last */
+        u32 index = 0;
+        if (in) index = atomicAdd(&place[bucket], 1u);
         __syncthreads();
-        return rank;
-    }
-    for (u32 k = 2u; k <= size; k <<= 1) {
-        for (u32 j = k >> 1; j > 0u; j >>= 1) {
-            u64 other;
-            if (j >= 64u) {
-                buf[t] = rank;
-                __syncthreads();
-                other = buf[t ^ j];
-                __syncthreads();
-            } else {
-                other = shfl_xor64(rank, (int)j);
-            }
-            /* the lower place of a pair keeps the larger value in runs that descend */
-            const bool larger = ((t & j) == 0u) == ((t & k) == 0u);
-            rank = (other > rank) == larger ? other : rank;
+        u64 all;
+        sm.start[t] = (u32)block_before(place[t], sm.red, all);
+        __syncthreads();
+        u32 at = 0, many = 0;
+        if (in) {
+            at = sm.start[bucket];
+            many = place[bucket];
+            buf[at + index] = rank;
         }
+        __syncthreads();
+        u32 before = at;
+        for (u32 i = 0; i < many; ++i) before += buf[at + i] > rank ? 1u : 0u;
+        __syncthreads();
+        if (in) buf[before] = rank;
     }
+    __syncthreads();
+    rank = t < n ? buf[t] : 0ull;
+    __syncthreads();
     return rank;
 }
 
@@ -323,21 +364,84 @@ __device__ __forceinline__ float kth_largest(const u32 *tops, u32 groups, u32 k)
 }
 
 /* The rank of the last value that is kept, of the n listed ones in order (one a
- * thread), in front of which base_n values and base_w units stand; all: units
- * of all values that top-p sums. */
-__device__ __forceinline__ u64 cut(const Row &r, const double *tab, u64 rank, u32 n, bool use_k, u64 base_n, u64 base_w, u64 all, u64 *red, u64 *out) {
+ * thread, with its weight), in front of which base_n values and base_w units
+ * stand; all: units of all values that top-p sums.  last: how many of the
+ * listed ones are kept. */
+__device__ __forceinline__ u64 cut(const Row &r, u64 rank, double wd, u32 n, bool use_k, u64 base_n, u64 base_w, u64 all, u64 *red, u64 *out, u32 &last) {
     const u32 t = threadIdx.x;
     const bool in = t < n;
-    const u64 bn = base_n + t, w = in ? units(weight(r, tab, of_key((u32)(rank >> IDX_BITS)))) : 0ull;
+    const u64 bn = base_n + t, w = in ? units(wd) : 0ull;
     const bool in_k = in && (!use_k || bn < r.k);
     u64 sum;
     const u64 bw = base_w + block_before(in_k ? w : 0ull, red, sum);
     const double target = (double)r.p * (double)(use_k ? sum : all);
     const bool kept = in_k && (!r.use_p || bn == 0ull || (double)bw < target);
-    const u32 last = (u32)__syncthreads_count(kept);
+    last = (u32)__syncthreads_count(kept);
     if (t + 1u == last) *out = rank;
     __syncthreads();
     return *out;
+}
+
+__device__ __forceinline__ double target_of(const uocr_sample_args &a, u32 b, u64 all) {
+    const float u = a.uniform[b];
+    return (double)(u > 0.0f ? fminf(u, 0.99999994f) : 0.0f) * (double)all;
+}
+
+/* The token, where the n values of largest rank (one a thread) are all that
+ * top-k and top-p keep: in front of each stands the weight of lower ids, summed
+ * as `sorted` counts: over all of few, else by buckets of ids. */
+__device__ __forceinline__ void pick_listed(const uocr_sample_args &a, u32 b, const Row &r, u64 rank, double wd, u32 n, Shared &sm) {
+    const u32 t = threadIdx.x, id = IDX_MASK - (u32)(rank & IDX_MASK);
+    const u64 w = t < n && wd >= r.min_w ? units(wd) : 0ull;
+    const u32 bits = 32u - (u32)__builtin_clz(a.vocab | 1u), bucket = id >> (bits > 10u ? bits - 10u : 0u);
+    u32 *count = sm.place, *ids = sm.count;
+    u64 *sums = sm.weight, *ws = sm.weight + LIST;
+    static_assert(LIST == 1024 && BINS >= 2 * LIST, "buckets of ten bits");
+    count[t] = 0u;
+    sums[t] = 0ull;
+    u64 all, sum = 0;
+    if (n <= FEW) {
+        const u32 size = n <= 64u ? 64u : FEW, parts = LIST / size, part = t / size, e = t % size;
+        if (t < n) ids[t] = id, ws[t] = w;
+        (void)block_before(w, sm.red, all);
+        if (e < n) {
+            const u32 mine = ids[e], i1 = n * (part + 1u) / parts;
+            u64 here = 0;
+#pragma unroll 4
+            for (u32 i = n * part / parts; i < i1; ++i) here += ids[i] < mine ? ws[i] : 0ull;
+            if (here != 0ull) atomicAdd(&sums[e], here);
+        }
+        __syncthreads();
+        sum = sums[t];
+    } else {
+        __syncthreads();
+        u32 index = 0;
+        if (w != 0ull) {
+            index = atomicAdd(&count[bucket], 1u);
+            atomicAdd(&sums[bucket], w);
+        }
+        __syncthreads();
+        u64 kept;
+        const u64 in_front = block_before(sums[t], sm.red, all);
+        sm.start[t] = (u32)block_before(count[t], sm.red2, kept);
+        sums[t] = in_front;
+        __syncthreads();
+        u32 at = 0, many = 0;
+        if (w != 0ull) {
+            at = sm.start[bucket];
+            many = count[bucket];
+            sum = sums[bucket];
+            ids[at + index] = id;
+            ws[at + index] = w;
+        }
+        __syncthreads();
+        for (u32 i = 0; i < many; ++i) sum += ids[at + i] < id ? ws[at + i] : 0ull;
+    }
+    const double target = target_of(a, b, all);
+    if (w != 0ull && !((double)sum > target) && (double)(sum + w) > target) {
+        a.tokens[b] = (int32_t)id;
+        if (a.probs != nullptr) a.probs[b] = (float)((double)w / (double)all);
+    }
 }
 
 /* What is known of the value that ends a kept set: it lies in bin `bin`, its
@@ -405,7 +509,7 @@ __device__ u64 last_kept(const void *row, u32 vocab, const Row &r, Region g, dou
     });
     __syncthreads();
     const u32 n = sm.n;
-    const u64 rank = sorted(t < n ? sm.list[t] : 0ull, n, sm.list, sm.place);
+    const u64 rank = sorted(t < n ? sm.list[t] : 0ull, n, sm);
     const u64 w = t < n ? units(weight(r, sm.tab, of_key((u32)(rank >> IDX_BITS)))) : 0ull;
     u64 all;
     const u64 before = g.before + block_before(t >= n ? 0ull : WEIGHTED ? w : 1ull, sm.red, all);
@@ -420,61 +524,15 @@ __device__ u64 last_kept(const void *row, u32 vocab, const Row &r, Region g, dou
     return thr;
 }
 
-/* The first id whose running sum of kept units is over the target, in the step
- * that `sum` stands in front of; by one wavefront.
- * Returns whether it is there, and what stands in front of the next values. */
-template <bool F32, typename K>
-__device__ __forceinline__ bool pick(const uocr_sample_args &a, u32 b, const void *row, u32 step, float least, double target, u64 all, u64 &sum, K &&kept) {
-    const u32 lane = threadIdx.x & 63u;
-    float x[E];
-    lane_load<F32, false>(row, min(step * STEP + lane * E, a.vocab), a.vocab, x);
-    u64 s = 0;
-    values_from(least, step, x, [&](float v, u32 id) { s += kept(v, id); });
-    u64 at = sum + wave_before(s);
-    const u64 found = __ballot(s != 0ull && !((double)at > target) && (double)(at + s) > target);
-    sum = shfl64(at + s, 63);
-    if (found == 0ull) return false;
-    if (lane == (u32)__ffsll((long long)found) - 1u) {
-        bool done = false;
-        values_from(least, step, x, [&](float y, u32 id) {
-            const u64 v = kept(y, id);
-            at += v;
-            if (!done && v != 0ull && (double)at > target) {
-                done = true;
-                a.tokens[b] = (int32_t)id;
-                if (a.probs != nullptr) a.probs[b] = (float)((double)v / (double)all);
-            }
-        });
-    }
-    return true;
-}
-
-__device__ __forceinline__ double target_of(const uocr_sample_args &a, u32 b, u64 all) {
-    const float u = a.uniform[b];
-    return (double)(u > 0.0f ? fminf(u, 0.99999994f) : 0.0f) * (double)all;
-}
-
-/* Rows that are decided by their largest logit; true where this one is. */
-__device__ __forceinline__ bool greedy(const uocr_sample_args &a, u32 b, u64 max_rank, float temp) {
-    if (max_rank != 0ull && temp > 0.0f) return false;
-    if (threadIdx.x == 0u) {
-        a.tokens[b] = max_rank == 0ull ? 0 : (int32_t)(IDX_MASK - (u32)(max_rank & IDX_MASK));
-        if (a.probs != nullptr) a.probs[b] = max_rank == 0ull ? 0.0f : 1.0f;
-    }
-    return true;
-}
-
-__device__ __forceinline__ float temperature_of(const uocr_sample_args &a, u32 b) {
-    return a.temperature != nullptr ? a.temperature[b] : 1.0f;
+/* A row that is decided by its largest logit. */
+__device__ __forceinline__ void greedy(const uocr_sample_args &a, u32 b, u64 max_rank) {
+    a.tokens[b] = max_rank == 0ull ? 0 : (int32_t)(IDX_MASK - (u32)(max_rank & IDX_MASK));
+    if (a.probs != nullptr) a.probs[b] = max_rank == 0ull ? 0.0f : 1.0f;
 }
 
 /* The rank of the block's largest logit, from its lanes'. */
 __device__ __forceinline__ u64 largest(float best, u32 best_id, u64 *red) {
-    u64 rank = best_id == 0xffffffffu ? 0ull : rank_of(best, best_id);
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 v = shfl_xor64(rank, o);
-        rank = v > rank ? v : rank;
-    }
+    u64 rank = wave_max64(best_id == 0xffffffffu ? 0ull : rank_of(best, best_id));
     if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = rank;
     __syncthreads();
     for (u32 i = 0; i < blockDim.x / 64u; ++i) rank = red[i] > rank ? red[i] : rank;
@@ -482,19 +540,110 @@ __device__ __forceinline__ u64 largest(float best, u32 best_id, u64 *red) {
     return rank;
 }
 
-/* Units that a value brings to the kept sum: ranks from thr on, not below min_p. */
-__device__ __forceinline__ u64 kept_units(const Row &r, const double *tab, float least, u64 thr, float x, u32 id) {
-    if (x == least && rank_of(x, id) < thr) return 0ull;
+/* What is kept: logits above `least`, and of those equal to it the ids up to
+ * `id`, if their weights are not below min_p.  raw: `least` as it stands in the
+ * row (with +inf logits, which are taken as 0, those alone). */
+struct Keep {
+    float least, raw;
+    u32 id;
+};
+__device__ __forceinline__ Keep keep_from(const Row &r, u64 thr) {
+    Keep k = {r.cut, 0.0f, IDX_MASK};
+    const float last = of_key((u32)(thr >> IDX_BITS));
+    if (thr != 0ull && last >= r.cut) k.least = last, k.id = IDX_MASK - (u32)(thr & IDX_MASK);
+    k.raw = r.inf ? INFINITY : k.least;
+    return k;
+}
+__device__ __forceinline__ bool is_kept(const Keep &k, float x, u32 id) {
+    return (x > k.least) | ((x == k.least) & (id <= k.id)); /* no branches */
+}
+
+/* Units that a value brings to the kept sum. */
+__device__ __forceinline__ u64 kept_units(const Row &r, const double *tab, const Keep &k, float raw, u32 id) {
+    const float x = value_of(r, raw);
+    if (!is_kept(k, x, id)) return 0ull;
     const double w = weight(r, tab, x);
     return w >= r.min_w ? units(w) : 0ull;
 }
-/* The logit below which nothing is kept (with +inf ones, as they stand in the
- * row: those alone). */
-__device__ __forceinline__ float least_of(const Row &r, u64 thr) {
-    return thr == 0ull ? r.cut : fmaxf(r.cut, of_key((u32)(thr >> IDX_BITS)));
+/* Those of the lane's values, of ids from id0 on.  Without branches: where few
+ * lanes have one the step is one of few, where many have one it takes half the
+ * instructions.  A loop: the code of a kernel is fetched by every CU. */
+__device__ __forceinline__ u64 lane_units(const Row &r, const double *tab, const Keep &k, u32 id0, const float *values) {
+    float x[E];
+#pragma unroll
+    for (u32 e = 0; e < E; ++e) x[e] = values[e];
+    if (r.inf) {
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) x[e] = value_of(r, x[e]);
+    }
+    u64 sum = 0;
+#pragma unroll 1
+    for (u32 e = 0; e < E; e += ILP) {
+#pragma unroll
+        for (u32 i = 0; i < ILP; ++i) {
+            const double w = weight(r, tab, is_kept(k, x[i], id0 + e + i) ? x[i] : -INFINITY);
+            sum += units(w >= r.min_w ? w : 0.0);
+        }
+#pragma unroll
+        for (u32 i = 0; i + ILP < E; ++i) x[i] = x[i + ILP];
+    }
+    return sum;
 }
-__device__ __forceinline__ float least_raw(const Row &r, float least) {
-    return r.inf ? INFINITY : least;
+
+/* The lane's values into the histogram (the last bin's have no weight): counts
+ * from `counted` bins, weights for top-p. */
+__device__ __forceinline__ void into_bins(const Row &r, const double *tab, const float *x, u32 counted, u32 *counts, u64 *weights) {
+    float v[E];
+#pragma unroll
+    for (u32 e = 0; e < E; ++e) v[e] = x[e];
+    if (r.inf) {
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) v[e] = value_of(r, v[e]);
+    }
+#pragma unroll 1
+    for (u32 e = 0; e < E; e += ILP) {
+        u32 bin[ILP];
+        u64 w[ILP];
+#pragma unroll
+        for (u32 i = 0; i < ILP; ++i) bin[i] = bin_of(r, v[i]);
+        if (r.use_p) {
+#pragma unroll
+            for (u32 i = 0; i < ILP; ++i) w[i] = units(weight(r, tab, v[i]));
+#pragma unroll
+            for (u32 i = 0; i < ILP; ++i)
+                if (bin[i] != BINS - 1u) atomicAdd(&weights[bin[i]], w[i]);
+        }
+#pragma unroll
+        for (u32 i = 0; i < ILP; ++i)
+            if (bin[i] < counted) atomicAdd(&counts[bin[i]], 1u);
+#pragma unroll
+        for (u32 i = 0; i + ILP < E; ++i) v[i] = v[i + ILP];
+    }
+}
+
+/* The first id whose running sum of kept units is over the target, in the step
+ * that `sum` stands in front of; by one wavefront: its lane by the steps' order,
+ * then that lane's values by a lane each.  Returns whether it is there, and what
+ * stands in front of the next values. */
+template <bool F32>
+__device__ __forceinline__ bool pick(const uocr_sample_args &a, u32 b, const Row &r, const double *tab, const Keep &k, const void *row, u32 step, double target, u64 all, u64 &sum) {
+    const u32 lane = threadIdx.x & 63u, id0 = step * STEP + lane * E;
+    float x[E];
+    lane_load<F32, false>(row, min(id0, a.vocab), a.vocab, x);
+    const u64 s = lane_units(r, tab, k, id0, x);
+    const u64 at = sum + wave_before(s);
+    const u64 found = __ballot(s != 0ull && !((double)at > target) && (double)(at + s) > target);
+    sum = lane64(at + s, 63);
+    if (found == 0ull) return false;
+    const u32 from = (u32)__builtin_ctzll(found), id = step * STEP + from * E + lane;
+    u64 w = 0;
+    if (lane < E && id < a.vocab) w = kept_units(r, tab, k, F32 ? ((const float *)row)[id] : (float)((const _Float16 *)row)[id], id);
+    const u64 before = lane64(at, (int)from) + wave_before(w);
+    if (w != 0ull && !((double)before > target) && (double)(before + w) > target) {
+        a.tokens[b] = (int32_t)id;
+        if (a.probs != nullptr) a.probs[b] = (float)((double)w / (double)all);
+    }
+    return true;
 }
 
 /* A row in one block.  The kept set of top-k and top-p is all values from some
@@ -516,10 +665,13 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
         if (lane == 0u) sm.tops[s % TOPS] = max(sm.tops[s % TOPS], top); /* a group's steps are one wavefront's: TOPS is a multiple of WAVES */
     });
     const u64 max_rank = largest(best, best_id, sm.red);
-    const float temp = temperature_of(a, b);
-    if (greedy(a, b, max_rank, temp)) return;
-    const Row r = row_of(a, b, max_rank, temp, shift);
-    fill_table(sm.tab);
+    Row r = settings_of(a, b, shift);
+    if (max_rank == 0ull || !r.hot) {
+        if (t == 0u) greedy(a, b, max_rank);
+        return;
+    }
+    set_top(r, max_rank);
+    fill_table(sm.tab, r.shift);
     if (t == 0u) sm.n = 0u;
     __syncthreads();
 
@@ -537,19 +689,20 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
         __syncthreads();
         const u32 n = sm.n;
         found = n <= LIST;
-        if (found) thr = cut(r, sm.tab, sorted(t < n ? sm.list[t] : 0ull, n, sm.list, sm.place), n, true, 0ull, 0ull, 0ull, sm.red, &sm.out[0]);
+        if (found) {
+            const u64 rank = sorted(t < n ? sm.list[t] : 0ull, n, sm);
+            const double wd = weight(r, sm.tab, of_key((u32)(rank >> IDX_BITS)));
+            u32 last;
+            thr = cut(r, rank, wd, n, true, 0ull, 0ull, 0ull, sm.red, &sm.out[0], last);
+            pick_listed(a, b, r, rank, wd, last, sm);
+            return;
+        }
         __syncthreads();
     }
     if (!found && (r.use_k || r.use_p)) {
         for (u32 i = t; i < BINS; i += NT) sm.weight[i] = 0ull, sm.count[i] = 0u;
         __syncthreads();
-        row_values<F32>(row, vocab, -INFINITY, [&](float raw, u32 id) {
-            const float x = value_of(r, raw);
-            const u32 i = bin_of(r, x);
-            if (i == BINS - 1u) return; /* no weight */
-            atomicAdd(&sm.count[i], 1u);
-            if (r.use_p) atomicAdd(&sm.weight[i], units(weight(r, sm.tab, x)));
-        });
+        each_step<F32, ROW_U>(row, vocab, wave, steps, WAVES, [&](u32, const float *x) { into_bins(r, sm.tab, x, BINS - 1u, sm.count, sm.weight); });
         __syncthreads();
         const u32 n0 = sm.count[2 * t], n1 = sm.count[2 * t + 1];
         const u64 w0 = sm.weight[2 * t], w1 = sm.weight[2 * t + 1];
@@ -585,17 +738,14 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
 
     /* the kept weights by id: a run of the row for each wavefront, a sum for each group of its steps */
     const u32 run = (steps + WAVES - 1u) / WAVES, per = (run + GROUPS - 1u) / GROUPS;
-    const float least = least_of(r, thr), raw_least = least_raw(r, least);
-    auto kept = [&](float raw, u32 id) { return kept_units(r, sm.tab, least, thr, value_of(r, raw), id); };
+    const Keep keep = keep_from(r, thr);
     u64 *sums = sm.weight; /* [WAVES][GROUPS] */
     __syncthreads();
     sums[t] = 0ull;
     __syncthreads();
     each_step<F32, ROW_U>(row, vocab, min(wave * run, steps), min(wave * run + run, steps), 1u, [&](u32 s, const float *x) {
-        u64 sum = 0;
-        values_from(raw_least, s, x, [&](float v, u32 id) { sum += kept(v, id); });
-        if (!__any(sum != 0ull)) return;
-        sum = wave_sum64(sum);
+        if (!__any(largest_of(x) >= keep.raw)) return;
+        const u64 sum = wave_sum64(lane_units(r, sm.tab, keep, s * STEP + lane * E, x));
         if (lane == 0u) sums[wave * GROUPS + (s - wave * run) / per] += sum;
     });
     __syncthreads();
@@ -610,7 +760,7 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
         const u32 w = (u32)sm.out[0] / GROUPS, g = (u32)sm.out[0] % GROUPS;
         u64 sum = sm.out[1];
         for (u32 i = g * per; i < min(g * per + per, run); ++i)
-            if (w * run + i < steps && pick<F32>(a, b, row, w * run + i, raw_least, target, all, sum, kept)) break;
+            if (w * run + i < steps && pick<F32>(a, b, r, sm.tab, keep, row, w * run + i, target, all, sum)) break;
     }
 }
 
@@ -627,18 +777,24 @@ __global__ __launch_bounds__(NT) void k_sample_row(uocr_sample_args a, u32 shift
 
 /* ---- a row over several blocks --------------------------------------------------- */
 
-/* What the histogram says of a row: whether its kept set ends (any), in a list
- * of n values that base_n values and base_w units stand in front of. */
+/* What is known of a row before its list is made: whether its kept set ends
+ * (any), in the values from `floor` on that lie in the bins first .. last (all
+ * for a bounded row), in front of which base_n values and base_w units stand;
+ * all_w: units of all values; crowded: more than LIST values, as far as they
+ * were counted. */
 struct Found {
     u64 base_n, base_w, all_w;
-    u32 n, any, use_k, pad;
+    u32 first, last;
+    float floor;
+    bool any, use_k, crowded;
 };
 
 /* What the launches of a row leave for each other, in the workspace. */
 struct Plan {
     uocr_sample_args a;
     u32 shift, steps, chunks;      /* of a row; chunks: of the first launch */
-    u32 parts, run;                /* of this launch: blocks of a row, steps of each */
+    u32 parts, run;                /* of this launch, [parts][rows] blocks: steps of each */
+    Row *settings;                 /* [rows] */
     u64 *max_rank;                 /* [rows][chunks] */
     u32 *tops;                     /* [rows][steps]: keys of the steps' largest logits */
     u64 *weight;                   /* [rows][BINS] */
@@ -646,35 +802,139 @@ struct Plan {
     u64 *list;                     /* [rows][LIST] */
     u32 *n;                        /* [rows]: the list's length so far */
     Found *found;                  /* [rows] */
-    u64 *thr;                      /* [rows]: the rank that ends the kept set */
+    u64 *thr;                      /* [rows]: the rank that ends the kept set, or DONE */
     u64 *sums;                     /* [rows][steps] */
+    u32 *arrived;                  /* [rows]: blocks that have written their sums */
     bool cut;                      /* some row has top-k or top-p */
 };
 
-template <bool F32, typename F>
-__device__ __forceinline__ void chunk_steps(const Plan &g, const void *row, u32 chunk, F &&f) {
-    each_step<F32, 4>(row, g.a.vocab, chunk * g.run + (threadIdx.x >> 6), min(chunk * g.run + g.run, g.steps), CWAVES, f);
+/* The lane's values of a step, as they stand in memory.  The row's last lanes,
+ * whose values may not be E, begin at its last E ones instead. */
+template <bool F32>
+struct Raw {
+    uint4 w[F32 ? 2 : 1];
+};
+__device__ __forceinline__ u32 lane_id0(u32 step, u32 vocab) { return min(step * STEP + (threadIdx.x & 63u) * E, vocab - E); }
+template <bool F32>
+__device__ __forceinline__ Raw<F32> raw_load(const void *row, u32 id0) {
+    Raw<F32> q;
+    if constexpr (F32) {
+        const f32x4_any4 a = *(const f32x4_any4 *)((const float *)row + id0), b = *(const f32x4_any4 *)((const float *)row + id0 + 4);
+        q.w[0] = __builtin_bit_cast(uint4, a);
+        q.w[1] = __builtin_bit_cast(uint4, b);
+    } else {
+        q.w[0] = load_any((const uint16_t *)row + id0);
+    }
+    return q;
 }
-template <bool F32, typename F>
-__device__ __forceinline__ void chunk_values(const Plan &g, const void *row, u32 chunk, float least, F &&f) {
-    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) { values_from(least, s, x, f); });
+/* NaN, which takes part in nothing, for those that are not of the lane. */
+template <bool F32>
+__device__ __forceinline__ void raw_values(const Raw<F32> &q, u32 step, u32 vocab, float *x) {
+    if constexpr (F32) {
+        const uint4 a = q.w[0], b = q.w[1];
+        const u32 v[E] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) x[e] = __uint_as_float(v[e]);
+    } else {
+        union {
+            uint4 u;
+            _Float16 h[E];
+        } v;
+        v.u = q.w[0];
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) x[e] = (float)v.h[e];
+    }
+    if ((step + 1u) * STEP > vocab) {
+        const u32 first = step * STEP + (threadIdx.x & 63u) * E - lane_id0(step, vocab);
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) x[e] = e < first ? __builtin_nanf("") : x[e];
+    }
+}
+
+/* The steps of a wavefront (every CWAVES-th of its chunk's), a lane each.  The
+ * first 64 are asked for their largest logits before anything else is known of
+ * the row: the launches below are chains of loads that wait for each other. */
+struct Steps {
+    const u32 *tops;
+    u32 s0, s1, key;
+};
+__device__ __forceinline__ Steps steps_of(const Plan &g, u32 b, u32 chunk) {
+    Steps c;
+    c.tops = g.tops + (u64)b * g.steps;
+    c.s0 = chunk * g.run + (u32)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    c.s1 = min(chunk * g.run + g.run, g.steps);
+    const u32 mine = c.s0 + CWAVES * (threadIdx.x & 63u);
+    c.key = mine < c.s1 ? c.tops[mine] : 0u;
+    return c;
+}
+
+/* f(step, first id, values) for the steps that hold a value from `least` on,
+ * four steps' loads at a time; skip(step) for the others, by a lane each. */
+template <bool F32, typename F, typename S>
+__device__ __forceinline__ void chunk_steps(const Plan &g, const void *row, const Steps &c, float least, F &&f, S &&skip) {
+    constexpr u32 U = 4;
+    const u32 lane = threadIdx.x & 63u, vocab = g.a.vocab, key = key_of(least), s1 = c.s1;
+#pragma unroll 1
+    for (u32 first = c.s0; first < s1; first += 64u * CWAVES) {
+        const u32 mine = first + CWAVES * lane;
+        const bool in = mine < s1, look = in && (first == c.s0 ? c.key : c.tops[mine]) >= key;
+        if (in && !look) skip(mine);
+        u64 left = __ballot(look);
+#pragma unroll 1
+        while (left != 0ull) {
+            u32 s[U], n = 0;
+            Raw<F32> q[U];
+#pragma unroll
+            for (u32 u = 0; u < U; ++u) {
+                s[u] = left != 0ull ? first + CWAVES * (u32)__builtin_ctzll(left) : s[u > 0u ? u - 1u : 0u]; /* the last one again */
+                n += left != 0ull ? 1u : 0u;
+                left &= left - 1ull;
+                q[u] = raw_load<F32>(row, lane_id0(s[u], vocab));
+            }
+#pragma unroll 1
+            for (u32 u = 0; u < n; ++u) {
+                float x[E];
+                raw_values<F32>(q[0], s[0], vocab, x);
+                f(s[0], lane_id0(s[0], vocab), x);
+#pragma unroll
+                for (u32 i = 0; i + 1u < U; ++i) q[i] = q[i + 1u], s[i] = s[i + 1u];
+            }
+        }
+    }
+}
+/* g(logit, id) for those values, up to `most`. */
+template <bool F32, typename G>
+__device__ __forceinline__ void chunk_values(const Plan &g, const void *row, const Steps &c, float least, float most, G &&each) {
+    chunk_steps<F32>(g, row, c, least, [&](u32, u32 id0, const float *x) {
+        u32 here = 0;
+#pragma unroll
+        for (u32 e = 0; e < E; ++e) here |= ((x[e] >= least) & (x[e] <= most)) ? 1u << e : 0u;
+        while (here != 0u) {
+            const u32 e = (u32)__builtin_ctz(here);
+            here &= here - 1u;
+            const float a0 = e & 1u ? x[1] : x[0], a1 = e & 1u ? x[3] : x[2], a2 = e & 1u ? x[5] : x[4], a3 = e & 1u ? x[7] : x[6];
+            const float c0 = e & 2u ? a1 : a0, c1 = e & 2u ? a3 : a2;
+            each(e & 4u ? c1 : c0, id0 + e);
+        }
+    }, [](u32) {});
 }
 
 /* 1: the steps' and the chunk's largest logit; the row's histogram is cleared. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_max(Plan g) {
     __shared__ u64 red[CWAVES];
-    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, lane = threadIdx.x & 63u;
+    const u32 b = blockIdx.x, chunk = blockIdx.y, lane = threadIdx.x & 63u;
     if (g.cut)
         for (u32 i = chunk * CT + threadIdx.x; i < BINS; i += CT * g.parts) g.weight[(u64)b * BINS + i] = 0ull, g.count[(u64)b * BINS + i] = 0u;
     if (chunk == 0u && threadIdx.x == 0u) {
-        g.n[b] = 0u;
+        g.settings[b] = settings_of(g.a, b, g.shift);
+        g.n[b] = g.arrived[b] = 0u;
         g.found[b] = Found{};
     }
     const void *row = row_at<F32>(g.a, b);
     float best = -INFINITY;
     u32 best_id = 0xffffffffu;
-    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) {
+    each_step<F32, 4>(row, g.a.vocab, chunk * g.run + (threadIdx.x >> 6), min(chunk * g.run + g.run, g.steps), CWAVES, [&](u32 s, const float *x) {
         const float top = step_largest(s, x, best, best_id);
         if (lane == 0u) g.tops[(u64)b * g.steps + s] = key_of(top);
     });
@@ -683,53 +943,39 @@ __global__ __launch_bounds__(CT) void k_sample_max(Plan g) {
 }
 
 __device__ __forceinline__ u64 row_max(const Plan &g, u32 b) {
-    u64 rank = (threadIdx.x & 63u) < g.chunks ? g.max_rank[(u64)b * g.chunks + (threadIdx.x & 63u)] : 0ull;
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 v = shfl_xor64(rank, o);
-        rank = v > rank ? v : rank;
-    }
-    return rank;
+    return wave_max64((threadIdx.x & 63u) < g.chunks ? g.max_rank[(u64)b * g.chunks + (threadIdx.x & 63u)] : 0ull);
 }
 
-/* 2: the histogram, in LDS and from there into the row's. */
-template <bool F32>
-__global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
-    __shared__ double tab[TAB];
-    __shared__ u64 weights[BINS];
-    __shared__ u32 counts[BINS];
-    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts;
-    const u64 max_rank = row_max(g, b);
-    const float temp = temperature_of(g.a, b);
-    if (max_rank == 0ull || !(temp > 0.0f)) return;
-    const Row r = row_of(g.a, b, max_rank, temp, g.shift);
-    if ((!r.use_k && !r.use_p) || bounded(r, min(g.steps, TOPS))) return;
-    for (u32 i = threadIdx.x; i < BINS; i += CT) weights[i] = 0ull, counts[i] = 0u;
-    if (r.use_p) fill_table(tab);
-    __syncthreads();
-    chunk_values<F32>(g, row_at<F32>(g.a, b), chunk, -INFINITY, [&](float raw, u32 id) {
-        const float x = value_of(r, raw);
-        const u32 i = bin_of(r, x);
-        if (i == BINS - 1u) return;
-        atomicAdd(&counts[i], 1u);
-        if (r.use_p) atomicAdd(&weights[i], units(weight(r, tab, x)));
-    });
-    __syncthreads();
-    for (u32 i = threadIdx.x; i < BINS; i += CT) {
-        if (counts[i] == 0u) continue;
-        atomicAdd(&g.count[(u64)b * BINS + i], counts[i]);
-        if (r.use_p) atomicAdd(&g.weight[(u64)b * BINS + i], weights[i]);
-    }
+/* Below: in bins behind `last`, as a comparison tells (three bins' margin for
+ * their roundings). */
+__device__ __forceinline__ float floor_of(const Row &r, u32 last) {
+    const float floor = r.top - ((float)last + 3.0f) / r.scale;
+    return floor > -INFINITY && !r.inf ? floor : -INFINITY;
+}
+/* Above: in bins before `first`. */
+__device__ __forceinline__ float ceiling_of(const Row &r, u32 first) {
+    const float ceiling = r.top - ((float)first - 3.0f) / r.scale;
+    return first > 3u && !r.inf && ceiling == ceiling ? ceiling : INFINITY;
 }
 
-/* The bins whose values decide: those up to `last` (from `first`), in front of
- * which base_n values and base_w units stand, n values in all. */
-struct Deciding {
-    u32 first, last, n;
-    u64 base_n, base_w, all_w;
-    bool use_k, any;
-};
+__device__ __forceinline__ u64 agent_load(const u64 *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-__device__ __forceinline__ Deciding deciding(const Plan &g, u32 b, const Row &r, u64 *red, u64 *red2, u64 *out) {
+/* Whether this block is the last of its row to come here; what the others have
+ * written (with agent scope) is there for it. */
+__device__ __forceinline__ bool comes_last(u32 *count, u32 parts, u32 *shared) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (parts == 1u) return true;
+    if (threadIdx.x == 0u) *shared = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const bool last = *shared == parts - 1u;
+    asm volatile("" ::: "memory");
+    return last;
+}
+
+/* The bins whose values decide, from the row's histogram; by each block for
+ * itself (done once, by the last block to add to it, it took 3 us more). */
+__device__ __forceinline__ Found find_bins(const Plan &g, u32 b, const Row &r, u64 *red, u64 *red2, u64 *out) {
     constexpr u32 PER = BINS / CT;
     const u32 t = threadIdx.x;
     u32 n[PER];
@@ -741,178 +987,189 @@ __device__ __forceinline__ Deciding deciding(const Plan &g, u32 b, const Row &r,
         sn += n[i];
         sw += w[i];
     }
-    u64 all_n, all_w;
-    u64 nb = block_before(sn, red, all_n), wb = block_before(sw, red2, all_w);
-    Deciding d;
-    d.all_w = all_w;
-    d.use_k = r.use_k && (u64)r.k < all_n;
-    d.any = d.use_k || r.use_p;
-    if (!d.any) return d;
-    const double target = (double)r.p * (double)all_w;
+    Found f = {};
+    u64 all_n;
+    u64 nb = block_before(sn, red, all_n), wb = block_before(sw, red2, f.all_w);
+    f.use_k = r.use_k && (u64)r.k < all_n;
+    f.any = f.use_k || r.use_p;
+    if (!f.any) return f; /* all are kept */
+    const double target = (double)r.p * (double)f.all_w;
 #pragma unroll
     for (u32 i = 0; i < PER; ++i) {
-        const bool here = d.use_k ? nb < r.k && r.k <= nb + n[i] : n[i] != 0u && (!(r.p > 0.0f) ? nb == 0ull : (double)wb < target && !((double)(wb + w[i]) < target));
+        const bool here = f.use_k ? nb < r.k && r.k <= nb + n[i] : w[i] != 0ull && (!(r.p > 0.0f) ? wb == 0ull : (double)wb < target && !((double)(wb + w[i]) < target));
         if (here) out[0] = PER * t + i, out[1] = nb, out[2] = wb, out[3] = n[i];
         nb += n[i];
         wb += w[i];
     }
     __syncthreads();
-    d.last = (u32)out[0];
-    /* with both, top-p decides within top-k's values: all of them are looked at */
-    const bool both = d.use_k && r.use_p;
-    d.first = both ? 0u : d.last;
-    d.base_n = both ? 0ull : out[1];
-    d.base_w = both ? 0ull : out[2];
-    const u64 count = both ? out[1] + out[3] : out[3];
-    d.n = count > LIST ? LIST + 1u : (u32)count;
-    return d;
+    f.last = (u32)out[0];
+    f.floor = floor_of(r, f.last);
+    /* With both, top-p decides within top-k's values: all of them are looked at.  As many as a list holds are listed from
+     * the first on: then nothing else needs to be looked at for the token. */
+    const bool known = r.use_k || f.last < COUNTED, all = (f.use_k && r.use_p) || (known && out[1] + out[3] <= LIST);
+    f.first = all ? 0u : f.last;
+    f.base_n = all ? 0ull : out[1];
+    f.base_w = all ? 0ull : out[2];
+    f.crowded = known && (all ? out[1] + out[3] : out[3]) > LIST;
+    return f;
 }
 
-/* 3: the values that decide, listed (in any order): those from top-k's bound on,
- * or those in the deciding bins. */
+/* 2: the histogram, in LDS and from there into the row's.  A bounded row only
+ * needs its bound. */
 template <bool F32>
-__global__ __launch_bounds__(CT) void k_sample_list(Plan g) {
-    __shared__ u64 red[CWAVES], red2[CWAVES], out[4], list[LIST];
-    __shared__ u32 n, first;
-    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, t = threadIdx.x;
+__global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
+    __shared__ double tab[TAB];
+    __shared__ u64 weights[BINS];
+    __shared__ u32 counts[BINS];
+    const u32 b = blockIdx.x, chunk = blockIdx.y, t = threadIdx.x, groups = min(g.steps, TOPS);
+    const Steps mine = steps_of(g, b, chunk);
+    Row r = g.settings[b];
+    fill_table(tab, g.shift);
+    if (!r.hot || (!r.use_k && !r.use_p)) return;
+    const bool listed = bounded(r, groups);
+    if (listed && (chunk != 0u || t >= 64u)) return;
     const u64 max_rank = row_max(g, b);
-    const float temp = temperature_of(g.a, b);
-    if (max_rank == 0ull || !(temp > 0.0f)) return;
-    const Row r = row_of(g.a, b, max_rank, temp, g.shift);
-    if (!r.use_k && !r.use_p) return;
-    if (t == 0u) n = 0u;
-    const u32 groups = min(g.steps, TOPS);
-    const void *row = row_at<F32>(g.a, b);
-    Found f = {};
-    f.any = 1u;
-    if (bounded(r, groups)) {
+    if (max_rank == 0ull) return;
+    set_top(r, max_rank);
+    if (listed) {
         u32 tops[TOPS / 64] = {};
         for (u32 s0 = 0; s0 < g.steps; s0 += TOPS) {
 #pragma unroll
             for (u32 i = 0; i < TOPS / 64; ++i) {
-                const u32 s = s0 + 64u * i + (t & 63u);
+                const u32 s = s0 + 64u * i + t;
                 if (s < g.steps) tops[i] = max(tops[i], g.tops[(u64)b * g.steps + s]);
             }
         }
-        const float floor = kth_largest(tops, groups, r.k);
-        __syncthreads();
-        f.use_k = 1u;
-        f.n = LIST;
-        if (chunk == 0u && t == 0u) g.found[b] = f;
-        chunk_values<F32>(g, row, chunk, floor, [&](float raw, u32 id) {
-            const u32 at = atomicAdd(&n, 1u);
-            if (at < LIST) list[at] = rank_of(value_of(r, raw), id);
-        });
-    } else {
-        const Deciding d = deciding(g, b, r, red, red2, out);
-        f.any = d.any ? 1u : 0u;
-        if (d.any) {
-            f.use_k = d.use_k ? 1u : 0u;
-            f.n = d.n;
-            f.base_n = d.base_n;
-            f.base_w = d.base_w;
-        }
-        f.all_w = d.all_w;
-        if (chunk == 0u && t == 0u) {
-            g.found[b] = f;
-            if (d.any && d.n > LIST) g.n[b] = LIST + 1u; /* too many */
-        }
-        if (!d.any || d.n > LIST) return;
-        /* most values are well below the deciding bins: a comparison tells (three bins' margin for the bins' roundings) */
-        float floor = r.top - ((float)d.last + 3.0f) / r.scale;
-        if (!(floor > -INFINITY) || r.inf) floor = -INFINITY;
-        chunk_values<F32>(g, row, chunk, floor, [&](float raw, u32 id) {
-            const float x = value_of(r, raw);
-            const u32 i = bin_of(r, x);
-            if (i < d.first || i > d.last) return;
-            const u32 at = atomicAdd(&n, 1u);
-            if (at < LIST) list[at] = rank_of(x, id); /* at most d.n: the bins were counted by the same arithmetic */
-        });
+        Found f = {};
+        f.any = f.use_k = true;
+        f.last = BINS;
+        f.floor = kth_largest(tops, groups, r.k);
+        if (t == 0u) g.found[b] = f;
+        return;
     }
+    for (u32 i = t; i < BINS; i += CT) weights[i] = 0ull, counts[i] = 0u;
     __syncthreads();
-    if (t == 0u && n != 0u) first = atomicAdd(&g.n[b], n); /* of a crowded list: past LIST */
+    const u32 counted = r.use_k ? BINS - 1u : COUNTED;
+    chunk_steps<F32>(g, row_at<F32>(g.a, b), mine, floor_of(r, BINS - 1u), [&](u32, u32, const float *x) { into_bins(r, tab, x, counted, counts, weights); }, [](u32) {});
+    __syncthreads();
+    for (u32 i = t; i < BINS; i += CT) {
+        if (counts[i] != 0u) atomicAdd(&g.count[(u64)b * BINS + i], counts[i]);
+        if (weights[i] != 0ull) atomicAdd(&g.weight[(u64)b * BINS + i], weights[i]);
+    }
+}
+
+/* 3: the values that decide, listed in any order. */
+template <bool F32>
+__global__ __launch_bounds__(CT) void k_sample_list(Plan g) {
+    __shared__ u64 red[CWAVES], red2[CWAVES], out[4], list[LIST];
+    __shared__ u32 n, first;
+    const u32 b = blockIdx.x, chunk = blockIdx.y, t = threadIdx.x;
+    const Steps mine = steps_of(g, b, chunk);
+    Row r = g.settings[b];
+    const u64 max_rank = row_max(g, b);
+    if (max_rank == 0ull || !r.hot || (!r.use_k && !r.use_p)) return;
+    set_top(r, max_rank);
+    if (t == 0u) n = 0u;
+    Found f;
+    if (bounded(r, min(g.steps, TOPS))) {
+        f = g.found[b];
+        __syncthreads();
+    } else {
+        f = find_bins(g, b, r, red, red2, out);
+        if (chunk == 0u && t == 0u) g.found[b] = f;
+        if (!f.any || f.crowded) return;
+    }
+    chunk_values<F32>(g, row_at<F32>(g.a, b), mine, f.floor, ceiling_of(r, f.first), [&](float raw, u32 id) {
+        const float x = value_of(r, raw);
+        const u32 i = bin_of(r, x);
+        if (f.last != BINS && (i < f.first || i > f.last)) return;
+        const u32 at = atomicAdd(&n, 1u);
+        if (at < LIST) list[at] = rank_of(x, id);
+    });
+    __syncthreads();
+    if (n == 0u) return;
+    if (t == 0u) first = atomicAdd(&g.n[b], n); /* of a crowded list: past LIST */
     __syncthreads();
     for (u32 i = t; i < min(n, LIST); i += CT)
         if (first + i < LIST) g.list[(u64)b * LIST + first + i] = list[i];
 }
 
 /* 4: the rank that ends the kept set: the listed values in order, what stands in
- * front of each, and the last one that is kept. */
+ * front of each, and the last one that is kept.  Where all of the kept set is
+ * listed, its token too; rows whose lists ran over are done from
+ * their beginning. */
 template <bool F32>
-__global__ __launch_bounds__(LIST) void k_sample_cut(Plan g) {
-    __shared__ double tab[TAB];
-    __shared__ u64 red[LIST / 64], list[LIST], out;
-    __shared__ u32 place[512];
+__global__ __launch_bounds__(NT) void k_sample_cut(Plan g) {
+    static_assert(LIST == NT, "a listed value for each thread");
+    __shared__ Shared sm;
     const u32 b = blockIdx.x, t = threadIdx.x;
-    const u64 max_rank = row_max(g, b);
-    const float temp = temperature_of(g.a, b);
-    if (max_rank == 0ull || !(temp > 0.0f)) return;
-    const Row r = row_of(g.a, b, max_rank, temp, g.shift);
+    Row r = g.settings[b];
     const Found f = g.found[b];
     const u32 n = g.n[b];
+    const u64 max_rank = row_max(g, b), listed = g.list[(u64)b * LIST + t];
+    if (max_rank == 0ull || !r.hot) return;
+    set_top(r, max_rank);
     u64 thr = 0;
-    if ((r.use_k || r.use_p) && f.any != 0u && n <= LIST) {
-        const u64 rank = t < n ? g.list[(u64)b * LIST + t] : 0ull;
-        fill_table(tab);
-        __syncthreads();
-        thr = cut(r, tab, sorted(rank, n, list, place), n, f.use_k != 0u, f.base_n, f.base_w, f.all_w, red, &out);
+    if (f.any) {
+        if (f.crowded || n > LIST) {
+            whole_row<F32>(g.a, b, row_at<F32>(g.a, b), g.shift, sm);
+            thr = DONE;
+        } else {
+            fill_table(sm.tab, r.shift);
+            __syncthreads();
+            const u64 rank = sorted(t < n ? listed : 0ull, n, sm);
+            const double wd = weight(r, sm.tab, of_key((u32)(rank >> IDX_BITS)));
+            u32 last;
+            thr = cut(r, rank, wd, n, f.use_k, f.base_n, f.base_w, f.all_w, sm.red, &sm.out[0], last);
+            if (f.base_n == 0ull) {
+                pick_listed(g.a, b, r, rank, wd, last, sm);
+                thr = DONE;
+            }
+        }
     }
     if (t == 0u) g.thr[b] = thr;
 }
 
-/* 5: the kept units of each step. */
+/* 5: the kept units of each step, from block to block with agent scope; the last
+ * block of a row finds the step, and in it the token. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_sums(Plan g) {
     __shared__ double tab[TAB];
-    const u32 b = blockIdx.x / g.parts, chunk = blockIdx.x % g.parts, t = threadIdx.x;
-    const u64 max_rank = row_max(g, b);
-    const float temp = temperature_of(g.a, b);
-    if (max_rank == 0ull || !(temp > 0.0f) || (g.cut && g.n[b] > LIST)) return;
-    const Row r = row_of(g.a, b, max_rank, temp, g.shift);
-    const u64 thr = g.cut ? g.thr[b] : 0ull;
-    fill_table(tab);
-    __syncthreads();
-    const void *row = row_at<F32>(g.a, b);
-    const float least = least_of(r, thr);
-    chunk_steps<F32>(g, row, chunk, [&](u32 s, const float *x) {
-        u64 sum = 0;
-        values_from(least_raw(r, least), s, x, [&](float raw, u32 id) { sum += kept_units(r, tab, least, thr, value_of(r, raw), id); });
-        if (__any(sum != 0ull)) sum = wave_sum64(sum);
-        if ((t & 63u) == 0u) g.sums[(u64)b * g.steps + s] = sum;
-    });
-}
-
-/* 6: the step that the target falls into, and its token.  Rows with crowded
- * bins are done here from the start. */
-template <bool F32>
-__global__ __launch_bounds__(NT) void k_sample_pick(Plan g) {
-    __shared__ Shared sm;
-    const u32 b = blockIdx.x, t = threadIdx.x;
-    const void *row = row_at<F32>(g.a, b);
-    const u64 max_rank = row_max(g, b);
-    const float temp = temperature_of(g.a, b);
-    if (greedy(g.a, b, max_rank, temp)) return;
-    if (g.cut && g.n[b] > LIST) {
-        whole_row<F32>(g.a, b, row, g.shift, sm);
+    __shared__ u64 red[CWAVES], at[2];
+    __shared__ u32 arrived;
+    const u32 b = blockIdx.x, chunk = blockIdx.y, t = threadIdx.x;
+    const Steps mine_steps = steps_of(g, b, chunk);
+    Row r = g.settings[b];
+    fill_table(tab, g.shift);
+    const u64 max_rank = row_max(g, b), thr = g.cut ? g.thr[b] : 0ull;
+    if (max_rank == 0ull || !r.hot) {
+        if (chunk == 0u && t == 0u) greedy(g.a, b, max_rank);
         return;
     }
-    const Row r = row_of(g.a, b, max_rank, temp, g.shift);
-    fill_table(sm.tab);
-    const u64 thr = g.cut ? g.thr[b] : 0ull;
-    const u32 per = (g.steps + NT - 1u) / NT, s0 = min(t * per, g.steps), s1 = min(s0 + per, g.steps);
+    if (thr == DONE) return;
+    set_top(r, max_rank);
+    const void *row = row_at<F32>(g.a, b);
+    __syncthreads();
+    const Keep keep = keep_from(r, thr);
+    u64 *sums = g.sums + (u64)b * g.steps;
+    auto put = [&](u32 s, u64 sum) { __hip_atomic_store(sums + s, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    chunk_steps<F32>(g, row, mine_steps, keep.raw, [&](u32 s, u32 id0, const float *x) {
+        const u64 sum = wave_sum64(lane_units(r, tab, keep, id0, x));
+        if ((t & 63u) == 0u) put(s, sum);
+    }, [&](u32 s) { put(s, 0ull); });
+    if (!comes_last(g.arrived + b, g.parts, &arrived)) return;
+    const u32 per = (g.steps + CT - 1u) / CT, s0 = min(t * per, g.steps), s1 = min(s0 + per, g.steps);
     u64 mine = 0;
-    for (u32 s = s0; s < s1; ++s) mine += g.sums[(u64)b * g.steps + s];
+    for (u32 s = s0; s < s1; ++s) mine += agent_load(sums + s);
     u64 all;
-    const u64 before = block_before(mine, sm.red, all);
+    const u64 before = block_before(mine, red, all);
     const double target = target_of(g.a, b, all);
-    if (mine != 0ull && !((double)before > target) && (double)(before + mine) > target) sm.out[0] = s0, sm.out[1] = before;
+    if (mine != 0ull && !((double)before > target) && (double)(before + mine) > target) at[0] = s0, at[1] = before;
     __syncthreads();
     if (t >= 64u) return;
-    const float least = least_of(r, thr);
-    auto kept = [&](float raw, u32 id) { return kept_units(r, sm.tab, least, thr, value_of(r, raw), id); };
-    u64 sum = sm.out[1];
-    for (u32 s = (u32)sm.out[0]; s < g.steps; ++s)
-        if (pick<F32>(g.a, b, row, s, least_raw(r, least), target, all, sum, kept)) break;
+    u64 sum = at[1];
+    for (u32 s = (u32)at[0]; s < g.steps; ++s)
+        if (pick<F32>(g.a, b, r, tab, keep, row, s, target, all, sum)) break;
 }
 
 u32 shift_of(u32 vocab) {
@@ -923,18 +1180,18 @@ u32 shift_of(u32 vocab) {
 
 /* Rows of up to ONE_BLOCK tokens are done by a block each, in one launch, and
  * with MANY_ROWS or more up to twice that: us by one launch and by several, fp16,
- * top-k alone and top-p alone, were 19 and 28 against 29 and 33 for 1 row of
- * 16,000, 23 and 39 against 29 and 34 for 1 of 32,000, 34 and 48 against 38 and
- * 47 for 64 of those, 49 and 80 against 55 and 80 for 192 of 64,000, 58 and 148
- * against 64 and 124 for 192 of 129,280. */
-constexpr u32 ONE_BLOCK = 16384, MANY_ROWS = 64;
+ * top-k alone and top-p alone, were 16 and 25 against 20 and 25 for 1 row of
+ * 16,000, 24 and 29 against 33 and 43 for 192; 19 and 36 against 21 and 25 for 1
+ * of 32,000, 33 and 44 against 29 and 41 for 64, 34 and 45 against 39 and 56 for
+ * 192; 51 and 74 against 46 and 74 for 192 of 64,000. */
+constexpr u32 ONE_BLOCK = 16384, MANY_ROWS = 128;
 bool by_one_block(u32 rows, u32 vocab) { return vocab <= (rows < MANY_ROWS ? ONE_BLOCK : 2u * ONE_BLOCK); }
 
 /* Blocks of a launch, all rows: where all values take little each, more of them
  * only have their own beginnings to pay for; where some rows' values take an
  * exponential and atomics each and others' nothing, the rows are cut finer.  192
- * mixed rows of 129,280 fp16 took 93.9 us so, 95.4 with 768 everywhere, 98.2 and
- * 96.8 with 1,400 and 4,096 for the heavy ones. */
+ * mixed rows of 129,280 fp16 took 88.7 us so (before their lists were ordered by
+ * buckets: 78.6), 91.1 and 91.7 with 1,536 and 3,000 for the heavy ones. */
 constexpr u32 LIGHT_BLOCKS = 768, HEAVY_BLOCKS = 2048;
 
 u32 parts_of(const Plan &g, u32 rows, u32 blocks) {
@@ -953,6 +1210,7 @@ size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
         at += (bytes + 255u) & ~(size_t)255u;
         return (void *)p;
     };
+    g.settings = (Row *)take((size_t)rows * sizeof(Row));
     g.max_rank = (u64 *)take((size_t)rows * MAX_CHUNKS * 8u);
     g.tops = (u32 *)take((size_t)rows * g.steps * 4u);
     g.weight = (u64 *)take((size_t)rows * BINS * 8u);
@@ -962,6 +1220,7 @@ size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
     g.found = (Found *)take((size_t)rows * sizeof(Found));
     g.thr = (u64 *)take((size_t)rows * 8u);
     g.sums = (u64 *)take((size_t)rows * g.steps * 8u);
+    g.arrived = (u32 *)take((size_t)rows * 4u);
     return at;
 }
 
@@ -978,16 +1237,15 @@ hipError_t launch(hipStream_t st, const uocr_sample_args &a) {
     auto go = [&](void (*kernel)(Plan), u32 blocks) {
         g.parts = parts_of(g, a.rows, blocks);
         g.run = (g.steps + g.parts - 1u) / g.parts;
-        hipLaunchKernelGGL(kernel, dim3(a.rows * g.parts), dim3(CT), 0, st, g);
+        hipLaunchKernelGGL(kernel, dim3(a.rows, g.parts), dim3(CT), 0, st, g);
     };
     go(k_sample_max<F32>, LIGHT_BLOCKS);
     if (g.cut) {
         go(k_sample_bins<F32>, HEAVY_BLOCKS);
         go(k_sample_list<F32>, LIGHT_BLOCKS);
-        hipLaunchKernelGGL((k_sample_cut<F32>), dim3(a.rows), dim3(LIST), 0, st, g);
+        hipLaunchKernelGGL((k_sample_cut<F32>), dim3(a.rows), dim3(NT), 0, st, g);
     }
     go(k_sample_sums<F32>, HEAVY_BLOCKS);
-    hipLaunchKernelGGL((k_sample_pick<F32>), dim3(a.rows), dim3(NT), 0, st, g);
     return hipGetLastError();
 }
 
