@@ -25,6 +25,15 @@ __device__ __forceinline__ uint4 load_once(const uint8_t *p) {
 constexpr u32 APPEND_TOKENS = 8; /* most tokens of a block */
 constexpr u32 APPEND_ITEMS = 1;  /* rows' pieces of a thread that are loaded at a time */
 
+/* The largest of a row's N lanes (4 or 8). */
+template <u32 N>
+__device__ __forceinline__ u32 row_max(u32 v) {
+    v = max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true)); /* quad_perm [1,0,3,2] */
+    v = max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true)); /* quad_perm [2,3,0,1] */
+    if (N == 8u) v = max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true)); /* row_half_mirror */
+    return v;
+}
+
 /* ---- append ----------------------------------------------------------------- */
 
 /* y1 = x1 cos - x2 sin, y2 = x1 sin + x2 cos on the pairs (i, i + D/2) of a
@@ -123,43 +132,46 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tp
             } else {
                 /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
                  * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8) */
-                float m0 = 0.0f, m1 = 0.0f;
+                /* the largest magnitudes by their bits: what is not finite is above all others */
+                u32 b0 = 0u, b1 = 0u;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    m0 = fabsf(y[e]) < INFINITY ? fmaxf(m0, fabsf(y[e])) : INFINITY;
-                    m1 = fabsf(y[8 + e]) < INFINITY ? fmaxf(m1, fabsf(y[8 + e])) : INFINITY;
+                    b0 = max(b0, __float_as_uint(y[e]) & 0x7fffffffu);
+                    b1 = max(b1, __float_as_uint(y[8 + e]) & 0x7fffffffu);
                 }
-                if (D == 64) m0 = m1 = fmaxf(m0, m1); /* both halves are one group */
-#pragma unroll
-                for (u32 o = 1; o < LPR; o <<= 1) {
-                    m0 = fmaxf(m0, __shfl_xor(m0, o));
-                    m1 = fmaxf(m1, __shfl_xor(m1, o));
-                }
-                union {
-                    int8_t b[8];
-                    uint2 u;
-                } q0, q1;
-                const float s0 = m0 == 0.0f ? 1.0f : m0 / 127.0f, s1 = m1 == 0.0f ? 1.0f : m1 / 127.0f;
+                if (D == 64) b0 = b1 = max(b0, b1); /* both halves are one group */
+                b0 = row_max<LPR>(b0);
+                b1 = row_max<LPR>(b1);
+                const bool f0 = b0 < 0x7f800000u, f1 = b1 < 0x7f800000u;
+                const float m0 = __uint_as_float(b0), m1 = __uint_as_float(b1);
+                const float s0 = b0 == 0u ? 1.0f : m0 / 127.0f, s1 = b1 == 0u ? 1.0f : m1 / 127.0f;
                 /* y / s rounded as a division is: the product with the rounded reciprocal, corrected by its residual
-                 * (Markstein's method; a quarter of a division's instructions, 28.9 against 30.9 us with the gather) */
+                 * (Markstein's method), then to the nearest integer by adding 1.5 2^23, in whose last byte it is left.  It
+                 * is 127 at most: scales are no subnormals (y is 0 or more than 2^-100), so their rounding adds 2^-23. */
                 const float i0 = 1.0f / s0, i1 = 1.0f / s1;
-                auto quotient = [](float v, float sc, float inv) {
+                auto quantised = [](float v, float sc, float inv) {
                     const float x = v * inv;
-                    return fmaf(fmaf(-x, sc, v), inv, x);
+                    return __float_as_uint(fmaf(fmaf(-x, sc, v), inv, x) + 12582912.0f);
                 };
+                auto bytes = [&](const float *v, float sc, float inv) {
+                    u32 w[2];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    /* a group that is not finite: 0 times its NaN scale */
-                    q0.b[e] = m0 < INFINITY ? (int8_t)fminf(fmaxf(rintf(quotient(y[e], s0, i0)), -127.0f), 127.0f) : (int8_t)0;
-                    q1.b[e] = m1 < INFINITY ? (int8_t)fminf(fmaxf(rintf(quotient(y[8 + e], s1, i1)), -127.0f), 127.0f) : (int8_t)0;
-                }
+                    for (int k = 0; k < 2; ++k) {
+                        const u32 q01 = __builtin_amdgcn_perm(quantised(v[4 * k + 1], sc, inv), quantised(v[4 * k], sc, inv), 0x0c0c0400u);
+                        const u32 q23 = __builtin_amdgcn_perm(quantised(v[4 * k + 3], sc, inv), quantised(v[4 * k + 2], sc, inv), 0x04000c0cu);
+                        w[k] = q01 | q23;
+                    }
+                    return make_uint2(w[0], w[1]);
+                };
+                /* a group that is not finite: 0 times its NaN scale */
+                const uint2 q0 = f0 ? bytes(y, s0, i0) : make_uint2(0u, 0u), q1 = f1 ? bytes(y + 8, s1, i1) : make_uint2(0u, 0u);
                 int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
-                *(uint2 *)dst = q0.u;
-                *(uint2 *)(dst + D / 2) = q1.u;
+                *(uint2 *)dst = q0;
+                *(uint2 *)(dst + D / 2) = q1;
                 if (lane == 0u) {
                     uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
-                    sc[0] = m0 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
-                    if (D == 128) sc[1] = m1 < INFINITY ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
+                    sc[0] = f0 ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
+                    if (D == 128) sc[1] = f1 ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
                 }
             }
         }
@@ -284,10 +296,6 @@ __device__ __forceinline__ u32 place(const Split &p, u32 b, uint64_t T0) {
     return p.q != 0u ? b : 2u * b + (share(p, b) >= T0 ? 0u : 1u);
 }
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    return ((uint64_t)(u32)__shfl_up((int)(v >> 32), d) << 32) | (u32)__shfl_up((int)v, d);
-}
-
 /* The split, and the tiles (padded) before the lane's run of sequences, by each
  * wavefront for itself. */
 __device__ __forceinline__ uint64_t make_split(const PagedGrid &g, u32 run, Split &p) {
@@ -297,14 +305,9 @@ __device__ __forceinline__ uint64_t make_split(const PagedGrid &g, u32 run, Spli
         own = padded(p, nt0);
         for (u32 s = s0 + 1u; s < s1; ++s) own += padded(p, len_tiles(seq_len(g.a, s)));
         own *= sets;
-        uint64_t all = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t v = shfl_up64(all, d);
-            if ((int)lane >= d) all += v;
-        }
-        p.total = (uint64_t)(u32)__builtin_amdgcn_readlane((int)all, 63) | ((uint64_t)(u32)__builtin_amdgcn_readlane((int)(all >> 32), 63) << 32);
-        return all - own;
+        const uint64_t all = wave_before(own);
+        p.total = lane64(own + all, 63);
+        return all;
     };
     p.q = 0u;
     uint64_t own, before = sum(own);
@@ -321,10 +324,6 @@ __device__ __forceinline__ uint64_t make_split(const PagedGrid &g, u32 run, Spli
     }
     p.blocks = (u32)min(n, (uint64_t)PA_BLOCKS); /* none without a tile */
     return before;
-}
-
-__device__ __forceinline__ uint64_t from_lane(uint64_t v, u32 lane) {
-    return (uint64_t)(u32)__builtin_amdgcn_readlane((int)v, (int)lane) | ((uint64_t)(u32)__builtin_amdgcn_readlane((int)(v >> 32), (int)lane) << 32);
 }
 
 /* The scale of group j, of two in a word. */
@@ -429,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
     /* the last lane whose run begins at or before tile lo has its sequence (each has a tile) */
     const u32 at_lane = 63u - (u32)__builtin_clzll(__ballot(before <= lo && lane * run < kv.n_seqs));
     u32 s = at_lane * run;
-    uint64_t base = from_lane(before, at_lane), at = lo;
+    uint64_t base = lane64(before, (int)at_lane), at = lo;
     uint8_t *vt = sm + wave * WLDS;
     while (at < hi) {
         const u32 len = seq_len(g.a, s), nt = len_tiles(len), ntp = padded(sp, nt);
@@ -709,7 +708,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedGrid g) {
     const u32 run = (kv.n_seqs + 63u) / 64u;
     const uint64_t before = make_split(g, run, sp);
     const u32 ntp = padded(sp, len_tiles(seq_len(g.a, s)));
-    uint64_t T0 = from_lane(before, s / run) + (uint64_t)set * ntp;
+    uint64_t T0 = lane64(before, (int)(s / run)) + (uint64_t)set * ntp;
     for (u32 i = s / run * run; i < s; ++i) T0 += (uint64_t)padded(sp, len_tiles(seq_len(g.a, i))) * sets;
     const u32 b0 = block_of(sp, T0), b1 = block_of(sp, T0 + ntp - 1u);
     if (b0 != b1) join_heads<D>(g, sp, T0, b0, b1, row, 1u, g.a.out + (uint64_t)s * g.a.os + h * D, sm);

@@ -4,7 +4,6 @@
 #include "uocr_dev.h"
 #include "uocr_serve.h"
 
-typedef unsigned long long u64;
 
 namespace {
 
@@ -212,17 +211,6 @@ __device__ __forceinline__ void row_values(const void *row, u32 vocab, float lea
     each_step<F32, ROW_U>(row, vocab, threadIdx.x >> 6, (vocab + STEP - 1u) / STEP, WAVES, [&](u32 s, const float *x) { values_from(least, s, x, f); });
 }
 
-__device__ __forceinline__ u64 lane64(u64 v, int lane) {
-    return ((u64)(u32)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (u32)__builtin_amdgcn_readlane((int)v, lane);
-}
-template <int CTRL>
-__device__ __forceinline__ u64 dpp64(u64 v) {
-    return ((u64)(u32)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true) << 32) |
-           (u32)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
-}
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int m) {
-    return ((u64)(u32)__shfl_xor((int)(v >> 32), m) << 32) | (u32)__shfl_xor((int)v, m);
-}
 /* Sum and maximum of all lanes (all of them active), as wave_sum. */
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
     v += dpp64<0xB1>(v);
@@ -237,19 +225,6 @@ __device__ __forceinline__ u64 wave_max64(u64 v) {
     v = max(v, dpp64<0x141>(v));
     v = max(v, dpp64<0x140>(v));
     return max(max(lane64(v, 0), lane64(v, 16)), max(lane64(v, 32), lane64(v, 48)));
-}
-
-/* Sums of what earlier lanes hold: row_shr by 1, 2, 4, 8 within 16 lanes (zeros
- * come in), then the rows'. */
-__device__ __forceinline__ u64 wave_before(u64 v) {
-    u64 s = v;
-    s += dpp64<0x111>(s);
-    s += dpp64<0x112>(s);
-    s += dpp64<0x114>(s);
-    s += dpp64<0x118>(s);
-    const u64 a = lane64(s, 15), b = a + lane64(s, 31), c = b + lane64(s, 47);
-    const u32 row = (threadIdx.x & 63u) >> 4;
-    return s - v + (row == 0u ? 0ull : row == 1u ? a : row == 2u ? b : c);
 }
 
 struct Shared {

@@ -95,6 +95,30 @@ __device__ __forceinline__ int kv_page(const uocr_kv &c, int32_t seq, uint32_t p
     return (uint32_t)p < c.n_pages ? p : -1;
 }
 
+typedef unsigned long long u64;
+
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+template <int CTRL>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+    return ((u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true) << 32) |
+           (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+
+/* Sums of what earlier lanes hold (all lanes are active): row_shr by 1, 2, 4, 8
+ * within 16 lanes, where zeros come in, then the rows'. */
+__device__ __forceinline__ u64 wave_before(u64 v) {
+    u64 s = v;
+    s += dpp64<0x111>(s);
+    s += dpp64<0x112>(s);
+    s += dpp64<0x114>(s);
+    s += dpp64<0x118>(s);
+    const u64 a = lane64(s, 15), b = a + lane64(s, 31), c = b + lane64(s, 47);
+    const uint32_t row = (threadIdx.x & 63u) >> 4;
+    return s - v + (row == 0u ? 0ull : row == 1u ? a : row == 2u ? b : c);
+}
+
 /* Rows that no alignment above a value's is known of: 16-byte loads and stores
  * at any value's boundary, which global memory instructions take. */
 typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
