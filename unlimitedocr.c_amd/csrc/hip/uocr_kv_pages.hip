@@ -23,6 +23,7 @@ __device__ __forceinline__ uint4 load_once(const uint8_t *p) {
 }
 
 constexpr u32 APPEND_TOKENS = 8; /* most tokens of a block */
+constexpr u32 GATHER_NT = 1024;  /* threads of a block */
 constexpr u32 APPEND_ITEMS = 1;  /* rows' pieces of a thread that are loaded at a time */
 
 /* The largest of a row's N lanes (4 or 8). */
@@ -180,51 +181,43 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tp
 
 /* ---- gather ------------------------------------------------------------------- */
 
-/* A copy (Q8_0: fp16(q * scale)), bound by HBM: 8 or 16 values a lane, four
- * items of a thread in flight. */
+/* A copy (Q8_0: fp16(q * scale)), bound by HBM: 8 or 16 values a lane, one item
+ * a thread.  Each item is a chain of loads (position, page, row) that only other
+ * wavefronts can hide, so no thread waits for a second one: 8,127 Q8_0 tokens of
+ * 10 heads took 34.0 us with four items a thread, 24.4 so (4.7 TB/s; 25.6 in
+ * blocks of 512 threads, 26.8 of 256). */
 template <int D, bool Q8>
-__global__ __launch_bounds__(256) void k_kv_gather(uocr_gather_args a, u32 tpb, bool once) {
-    constexpr u32 E = Q8 ? 16 : 8, LPR = D / E, U = 4;
-    const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
+__global__ __launch_bounds__(GATHER_NT) void k_kv_gather(uocr_gather_args a, u32 tpb, bool once) {
+    constexpr u32 E = Q8 ? 16 : 8, LPR = D / E;
+    const u32 t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
     const u32 kvh = a.kv.heads, first = a.k_out == nullptr ? kvh : 0u, rows = (a.v_out == nullptr ? kvh : 2u * kvh) - first;
     const u32 items = nt * rows * LPR;
-    for (u32 i0 = t; i0 < items; i0 += 256u * U) {
-        uint4 w[U];
-        u32 sc[U];
-#pragma unroll
-        for (u32 u = 0; u < U; ++u) {
-            const u32 i = i0 + 256u * u;
-            w[u] = make_uint4(0u, 0u, 0u, 0u);
-            sc[u] = 0u;
-            if (i >= items) continue;
-            const u32 lane = i % LPR, tok = t0 + i / LPR / rows, r = i / LPR % rows + first;
-            const int seq = a.seqs != nullptr ? a.seqs[tok] : (int)tok, pos = a.pos[tok];
-            if (seq < 0 || (u32)seq >= a.kv.n_seqs || pos < 0 || ((u32)pos >> a.kv.shift) >= a.kv.table_stride) continue;
-            const int page = kv_page(a.kv, seq, (u32)pos);
-            if (page < 0) continue;
-            const bool is_v = r >= kvh;
-            const u32 slot = ((is_v ? r - kvh : r) << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u));
+    for (u32 i = threadIdx.x; i < items; i += GATHER_NT) {
+        const u32 lane = i % LPR, tok = t0 + i / LPR / rows, r = i / LPR % rows + first;
+        const bool is_v = r >= kvh;
+        const u32 h = is_v ? r - kvh : r;
+        const int seq = a.seqs != nullptr ? a.seqs[tok] : (int)tok, pos = a.pos[tok];
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        u32 sc = 0u;
+        int page = -1;
+        if (seq >= 0 && (u32)seq < a.kv.n_seqs && pos >= 0 && ((u32)pos >> a.kv.shift) < a.kv.table_stride) page = kv_page(a.kv, seq, (u32)pos);
+        if (page >= 0) {
+            const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u));
             const uint64_t at = (uint64_t)page * a.kv.page_stride + (uint64_t)slot * D + E * lane;
             const uint8_t *src = (const uint8_t *)(is_v ? a.kv.v : a.kv.k) + (Q8 ? at : 2u * at);
-            w[u] = once ? load_once(src) : *(const uint4 *)src;
-            if (Q8) sc[u] = (is_v ? a.kv.vs : a.kv.ks)[(uint64_t)page * (a.kv.page_stride / 64u) + slot * (D / 64u) + lane / 4u];
+            w = once ? load_once(src) : *(const uint4 *)src;
+            if (Q8) sc = (is_v ? a.kv.vs : a.kv.ks)[(uint64_t)page * (a.kv.page_stride / 64u) + slot * (D / 64u) + lane / 4u];
         }
-#pragma unroll
-        for (u32 u = 0; u < U; ++u) {
-            const u32 i = i0 + 256u * u;
-            if (i >= items) continue;
-            const u32 lane = i % LPR, tok = t0 + i / LPR / rows, r = i / LPR % rows + first;
-            uint16_t *dst = r >= kvh ? a.v_out + tok * a.vos + (r - kvh) * D : a.k_out + tok * a.kos + r * D;
-            if constexpr (!Q8) {
-                store_any(dst + 8u * lane, w[u]);
-            } else {
-                U4H8 lo, hi;
-                /* an absent token's zeros are zeros with any scale: its payload 0 and scale 0 */
-                lo.v = dequant_q8(w[u].x, w[u].y, sc[u]);
-                hi.v = dequant_q8(w[u].z, w[u].w, sc[u]);
-                store_any(dst + 16u * lane, lo.u);
-                store_any(dst + 16u * lane + 8u, hi.u);
-            }
+        uint16_t *dst = (is_v ? a.v_out + tok * a.vos : a.k_out + tok * a.kos) + h * D + E * lane;
+        if constexpr (!Q8) {
+            store_any(dst, w);
+        } else {
+            U4H8 lo, hi;
+            /* an absent token's zeros are zeros with any scale: its payload 0 and scale 0 */
+            lo.v = dequant_q8(w.x, w.y, sc);
+            hi.v = dequant_q8(w.z, w.w, sc);
+            store_any(dst, lo.u);
+            store_any(dst + 8u, hi.u);
         }
     }
 }
@@ -734,18 +727,18 @@ hipError_t uocr_launch_kv_append(hipStream_t st, const uocr_append_args *a) {
 hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
     const u32 sides = (a->k_out != nullptr ? 1u : 0u) + (a->v_out != nullptr ? 1u : 0u);
     const u32 lanes = sides * a->kv.heads * a->kv.dim / (a->kv.q8 ? 16u : 8u);
-    const u32 tpb = lanes >= 1024u ? 1u : 1024u / lanes; /* 1,024 items: four of each thread */
-    /* Pages of many tokens are read past the caches (16,000 tokens of 8 heads of 128, eight caches in turn: fp16 29.8
-     * against 31.0 us, Q8_0 29.5 against 31.2), those of few may be there still (4,000 of 10: 9.9 against 12.9, 10.8
-     * against 12.8 with three in turn). */
+    const u32 tpb = lanes >= GATHER_NT ? 1u : GATHER_NT / lanes;
+    /* Pages of many tokens are read past the caches (16,000 tokens of 8 heads of 128, eight caches in turn: fp16 27.5
+     * against 27.9 us, Q8_0 24.2 against 25.4; 8,127 Q8_0 ones of 10: 25.6 against 28.4), those of few may be there still
+     * (4,000 of 10: 8.8 against 11.3, 8.4 against 9.6). */
     const bool once = (uint64_t)a->tokens * lanes * 16u > (24u << 20);
     const dim3 grid((a->tokens + tpb - 1u) / tpb);
     if (a->kv.dim == 128u) {
-        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<128, true>), grid, dim3(256), 0, st, *a, tpb, once);
-        else hipLaunchKernelGGL((k_kv_gather<128, false>), grid, dim3(256), 0, st, *a, tpb, once);
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<128, true>), grid, dim3(GATHER_NT), 0, st, *a, tpb, once);
+        else hipLaunchKernelGGL((k_kv_gather<128, false>), grid, dim3(GATHER_NT), 0, st, *a, tpb, once);
     } else {
-        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<64, true>), grid, dim3(256), 0, st, *a, tpb, once);
-        else hipLaunchKernelGGL((k_kv_gather<64, false>), grid, dim3(256), 0, st, *a, tpb, once);
+        if (a->kv.q8) hipLaunchKernelGGL((k_kv_gather<64, true>), grid, dim3(GATHER_NT), 0, st, *a, tpb, once);
+        else hipLaunchKernelGGL((k_kv_gather<64, false>), grid, dim3(GATHER_NT), 0, st, *a, tpb, once);
     }
     return hipGetLastError();
 }
