@@ -1216,7 +1216,9 @@ hipError_t launch(hipStream_t st, const uocr_sample_args &a) {
     };
     go(k_sample_max<F32>, LIGHT_BLOCKS);
     if (g.cut) {
-        go(k_sample_bins<F32>, HEAVY_BLOCKS);
+        /* a block adds up to 2,048 bins to its row's: 16 blocks a row where that fills the chip (64 rows with top-p: 17.8
+         * us, 24.2 with 32 a row; 1 row 7.0, so 5.7) */
+        go(k_sample_bins<F32>, a.rows * 16u < 256u ? 256u : a.rows * 16u < HEAVY_BLOCKS ? a.rows * 16u : HEAVY_BLOCKS);
         go(k_sample_list<F32>, LIGHT_BLOCKS);
         hipLaunchKernelGGL((k_sample_cut<F32>), dim3(a.rows), dim3(NT), 0, st, g);
     }
