@@ -24,7 +24,6 @@ __device__ __forceinline__ uint4 load_once(const uint8_t *p) {
 
 constexpr u32 APPEND_TOKENS = 8; /* most tokens of a block */
 constexpr u32 GATHER_NT = 1024;  /* threads of a block */
-constexpr u32 APPEND_ITEMS = 1;  /* rows' pieces of a thread that are loaded at a time */
 
 /* The largest of a row's N lanes (4 or 8). */
 template <u32 N>
@@ -46,10 +45,11 @@ __device__ __forceinline__ u32 row_max(u32 v) {
  * be off by 0.06 radians); a block computes them once per token, in LDS, for
  * all its heads. */
 /* 8 blocks of a CU: with the registers that the compiler takes by itself (3 blocks) 16,000 fp16 tokens of 32 + 8 heads
- * take 128 us, so 82 (5.2 TB/s, a large copy's rate). */
+ * take 128 us, so 82 (5.2 TB/s, a large copy's rate); blocks of 512 threads 88.  4,988 Q8_0 tokens of 10 + 20 heads take
+ * 22.9 (3.4 TB/s). */
 template <int D, bool Q8>
 __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tpb) {
-    constexpr u32 LPR = D / 16, U = APPEND_ITEMS;
+    constexpr u32 LPR = D / 16;
     __shared__ float2 cs[APPEND_TOKENS][D / 2];
     __shared__ int page_of[APPEND_TOKENS], pos_of[APPEND_TOKENS];
     const u32 t = threadIdx.x, t0 = blockIdx.x * tpb, nt = min(tpb, a.tokens - t0);
@@ -59,16 +59,12 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tp
         const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
         return (is_q ? a.q + (t0 + tok) * a.qs : is_v ? a.v + (t0 + tok) * a.vs : a.k + (t0 + tok) * a.ks) + h * D;
     };
-    uint4 raw[2 * U];
-    auto load = [&](u32 first) {
-#pragma unroll
-        for (u32 u = 0; u < U; ++u) {
-            const u32 i = first + 256u * u;
-            if (i >= items) continue;
-            const uint16_t *src = source(i / LPR / rows, i / LPR % rows) + 8u * (i % LPR);
-            raw[2 * u] = load_any(src);
-            raw[2 * u + 1] = load_any(src + D / 2);
-        }
+    uint4 raw0, raw1;
+    auto load = [&](u32 i) {
+        if (i >= items) return;
+        const uint16_t *src = source(i / LPR / rows, i / LPR % rows) + 8u * (i % LPR);
+        raw0 = load_any(src);
+        raw1 = load_any(src + D / 2);
     };
     load(t);
     if (a.rotate) {
@@ -89,91 +85,86 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tp
     }
     __syncthreads();
 #pragma unroll 1
-    for (u32 i0 = t; i0 < items; i0 += 256u * U) {
-        if (i0 != t) load(i0);
+    for (u32 i = t; i < items; i += 256u) {
+        if (i != t) load(i);
+        const u32 lane = i % LPR, tok = i / LPR / rows, r = i / LPR % rows;
+        const int pos = pos_of[tok];
+        if (pos < 0) continue; /* a padding row: the whole row's lanes leave together */
+        const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
+        const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
+        U4H8 lo, hi;
+        lo.u = raw0;
+        hi.u = raw1;
+        float y[16];
 #pragma unroll
-        for (u32 u = 0; u < U; ++u) {
-            const u32 i = i0 + 256u * u;
-            if (i >= items) continue;
-            const u32 lane = i % LPR, tok = i / LPR / rows, r = i / LPR % rows;
-            const int pos = pos_of[tok];
-            if (pos < 0) continue; /* a padding row: the whole row's lanes leave together */
-            const bool is_q = r < a.heads, is_v = r >= a.heads + kvh;
-            const u32 h = is_q ? r : r - a.heads - (is_v ? kvh : 0u);
-            U4H8 lo, hi;
-            lo.u = raw[2 * u];
-            hi.u = raw[2 * u + 1];
-            float y[16];
+        for (int e = 0; e < 8; ++e) {
+            const float x1 = (float)lo.h[e], x2 = (float)hi.h[e];
+            if (a.rotate && !is_v) {
+                const float2 w = cs[tok][8u * lane + e];
+                y[e] = fmaf(x1, w.x, -(x2 * w.y));
+                y[8 + e] = fmaf(x1, w.y, x2 * w.x);
+            } else {
+                y[e] = x1;
+                y[8 + e] = x2;
+            }
+            lo.h[e] = (h16)y[e];
+            hi.h[e] = (h16)y[8 + e];
+        }
+        uint16_t *rows_out = is_q ? a.q_out + (t0 + tok) * a.qos : is_v || a.k_out == nullptr ? nullptr : a.k_out + (t0 + tok) * a.kos;
+        if (rows_out != nullptr) {
+            store_any(rows_out + h * D + 8u * lane, lo.u);
+            store_any(rows_out + h * D + 8u * lane + D / 2, hi.u);
+        }
+        if (is_q || page_of[tok] < 0) continue;
+        const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u)); /* row of the page */
+        const uint64_t at = (uint64_t)page_of[tok] * a.kv.page_stride + (uint64_t)slot * D + 8u * lane;
+        if constexpr (!Q8) {
+            uint16_t *dst = (uint16_t *)(is_v ? a.kv.v : a.kv.k) + at;
+            *(uint4 *)dst = lo.u;
+            *(uint4 *)(dst + D / 2) = hi.u;
+        } else {
+            /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
+             * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8).  The
+             * largest magnitudes go by their bits: what is not finite is above all others. */
+            u32 b0 = 0u, b1 = 0u;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x1 = (float)lo.h[e], x2 = (float)hi.h[e];
-                if (a.rotate && !is_v) {
-                    const float2 w = cs[tok][8u * lane + e];
-                    y[e] = fmaf(x1, w.x, -(x2 * w.y));
-                    y[8 + e] = fmaf(x1, w.y, x2 * w.x);
-                } else {
-                    y[e] = x1;
-                    y[8 + e] = x2;
-                }
-                lo.h[e] = (h16)y[e];
-                hi.h[e] = (h16)y[8 + e];
+                b0 = max(b0, __float_as_uint(y[e]) & 0x7fffffffu);
+                b1 = max(b1, __float_as_uint(y[8 + e]) & 0x7fffffffu);
             }
-            uint16_t *rows_out = is_q ? a.q_out + (t0 + tok) * a.qos : is_v || a.k_out == nullptr ? nullptr : a.k_out + (t0 + tok) * a.kos;
-            if (rows_out != nullptr) {
-                store_any(rows_out + h * D + 8u * lane, lo.u);
-                store_any(rows_out + h * D + 8u * lane + D / 2, hi.u);
-            }
-            if (is_q || page_of[tok] < 0) continue;
-            const u32 slot = (h << a.kv.shift) + ((u32)pos & ((1u << a.kv.shift) - 1u)); /* row of the page */
-            const uint64_t at = (uint64_t)page_of[tok] * a.kv.page_stride + (uint64_t)slot * D + 8u * lane;
-            if constexpr (!Q8) {
-                uint16_t *dst = (uint16_t *)(is_v ? a.kv.v : a.kv.k) + at;
-                *(uint4 *)dst = lo.u;
-                *(uint4 *)(dst + D / 2) = hi.u;
-            } else {
-                /* the quantiser's rule from the fp32 values: scale = max / 127 (1 for zeros), q = rint(y / scale), the
-                 * scale then rounded to fp16 (2^-11; below 6e-5, values of under 0.008, to the subnormals' 3e-8) */
-                /* the largest magnitudes by their bits: what is not finite is above all others */
-                u32 b0 = 0u, b1 = 0u;
+            if (D == 64) b0 = b1 = max(b0, b1); /* both halves are one group */
+            b0 = row_max<LPR>(b0);
+            b1 = row_max<LPR>(b1);
+            const bool f0 = b0 < 0x7f800000u, f1 = b1 < 0x7f800000u;
+            const float m0 = __uint_as_float(b0), m1 = __uint_as_float(b1);
+            const float s0 = b0 == 0u ? 1.0f : m0 / 127.0f, s1 = b1 == 0u ? 1.0f : m1 / 127.0f;
+            /* y / s rounded as a division is: the product with the rounded reciprocal, corrected by its residual
+             * (Markstein's method), then to the nearest integer by adding 1.5 2^23, in whose last byte it is left.  It
+             * is 127 at most: scales are no subnormals (y is 0 or more than 2^-100), so their rounding adds 2^-23. */
+            const float i0 = 1.0f / s0, i1 = 1.0f / s1;
+            auto quantised = [](float v, float sc, float inv) {
+                const float x = v * inv;
+                return __float_as_uint(fmaf(fmaf(-x, sc, v), inv, x) + 12582912.0f);
+            };
+            auto bytes = [&](const float *v, float sc, float inv) {
+                u32 w[2];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    b0 = max(b0, __float_as_uint(y[e]) & 0x7fffffffu);
-                    b1 = max(b1, __float_as_uint(y[8 + e]) & 0x7fffffffu);
+                for (int k = 0; k < 2; ++k) {
+                    const u32 q01 = __builtin_amdgcn_perm(quantised(v[4 * k + 1], sc, inv), quantised(v[4 * k], sc, inv), 0x0c0c0400u);
+                    const u32 q23 = __builtin_amdgcn_perm(quantised(v[4 * k + 3], sc, inv), quantised(v[4 * k + 2], sc, inv), 0x04000c0cu);
+                    w[k] = q01 | q23;
                 }
-                if (D == 64) b0 = b1 = max(b0, b1); /* both halves are one group */
-                b0 = row_max<LPR>(b0);
-                b1 = row_max<LPR>(b1);
-                const bool f0 = b0 < 0x7f800000u, f1 = b1 < 0x7f800000u;
-                const float m0 = __uint_as_float(b0), m1 = __uint_as_float(b1);
-                const float s0 = b0 == 0u ? 1.0f : m0 / 127.0f, s1 = b1 == 0u ? 1.0f : m1 / 127.0f;
-                /* y / s rounded as a division is: the product with the rounded reciprocal, corrected by its residual
-                 * (Markstein's method), then to the nearest integer by adding 1.5 2^23, in whose last byte it is left.  It
-                 * is 127 at most: scales are no subnormals (y is 0 or more than 2^-100), so their rounding adds 2^-23. */
-                const float i0 = 1.0f / s0, i1 = 1.0f / s1;
-                auto quantised = [](float v, float sc, float inv) {
-                    const float x = v * inv;
-                    return __float_as_uint(fmaf(fmaf(-x, sc, v), inv, x) + 12582912.0f);
-                };
-                auto bytes = [&](const float *v, float sc, float inv) {
-                    u32 w[2];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const u32 q01 = __builtin_amdgcn_perm(quantised(v[4 * k + 1], sc, inv), quantised(v[4 * k], sc, inv), 0x0c0c0400u);
-                        const u32 q23 = __builtin_amdgcn_perm(quantised(v[4 * k + 3], sc, inv), quantised(v[4 * k + 2], sc, inv), 0x04000c0cu);
-                        w[k] = q01 | q23;
-                    }
-                    return make_uint2(w[0], w[1]);
-                };
-                /* a group that is not finite: 0 times its NaN scale */
-                const uint2 q0 = f0 ? bytes(y, s0, i0) : make_uint2(0u, 0u), q1 = f1 ? bytes(y + 8, s1, i1) : make_uint2(0u, 0u);
-                int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
-                *(uint2 *)dst = q0;
-                *(uint2 *)(dst + D / 2) = q1;
-                if (lane == 0u) {
-                    uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
-                    sc[0] = f0 ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
-                    if (D == 128) sc[1] = f1 ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
-                }
+                return make_uint2(w[0], w[1]);
+            };
+            /* a group that is not finite: 0 times its NaN scale */
+            const uint2 q0 = f0 ? bytes(y, s0, i0) : make_uint2(0u, 0u), q1 = f1 ? bytes(y + 8, s1, i1) : make_uint2(0u, 0u);
+            int8_t *dst = (int8_t *)(is_v ? a.kv.v : a.kv.k) + at;
+            *(uint2 *)dst = q0;
+            *(uint2 *)(dst + D / 2) = q1;
+            if (lane == 0u) {
+                uint16_t *sc = (is_v ? a.kv.vs : a.kv.ks) + (uint64_t)page_of[tok] * (a.kv.page_stride / 64u) + slot * (D / 64u);
+                sc[0] = f0 ? __builtin_bit_cast(uint16_t, (h16)s0) : (uint16_t)0x7e00u;
+                if (D == 128) sc[1] = f1 ? __builtin_bit_cast(uint16_t, (h16)s1) : (uint16_t)0x7e00u;
             }
         }
     }
@@ -183,8 +174,8 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(uocr_append_args a, u32 tp
 
 /* A copy (Q8_0: fp16(q * scale)), bound by HBM: 8 or 16 values a lane, one item
  * a thread.  Each item is a chain of loads (position, page, row) that only other
- * wavefronts can hide, so no thread waits for a second one: 8,127 Q8_0 tokens of
- * 10 heads took 34.0 us with four items a thread, 24.4 so (4.7 TB/s; 25.6 in
+ * wavefronts can hide, so no thread waits for a second one: 18,569 Q8_0 tokens of
+ * 8 heads took 34.0 us with four items a thread, 24.4 so (4.7 TB/s; 25.6 in
  * blocks of 512 threads, 26.8 of 256). */
 template <int D, bool Q8>
 __global__ __launch_bounds__(GATHER_NT) void k_kv_gather(uocr_gather_args a, u32 tpb, bool once) {
@@ -729,7 +720,7 @@ hipError_t uocr_launch_kv_gather(hipStream_t st, const uocr_gather_args *a) {
     const u32 lanes = sides * a->kv.heads * a->kv.dim / (a->kv.q8 ? 16u : 8u);
     const u32 tpb = lanes >= GATHER_NT ? 1u : GATHER_NT / lanes;
     /* Pages of many tokens are read past the caches (16,000 tokens of 8 heads of 128, eight caches in turn: fp16 27.5
-     * against 27.9 us, Q8_0 24.2 against 25.4; 8,127 Q8_0 ones of 10: 25.6 against 28.4), those of few may be there still
+     * against 27.9 us, Q8_0 24.2 against 25.4; 18,569 Q8_0 ones of 8: 25.6 against 28.4), those of few may be there still
      * (4,000 of 10: 8.8 against 11.3, 8.4 against 9.6). */
     const bool once = (uint64_t)a->tokens * lanes * 16u > (24u << 20);
     const dim3 grid((a->tokens + tpb - 1u) / tpb);

@@ -9,7 +9,8 @@ non-OK status (ffi.py:681-699), and a per-engine lock (ffi.py:691).
 
 MI355X additions: ``Engine.from_memory`` / ``Engine.generate_embeddings``
 (precomputed image rows, include/uocr_hip.h), the hot-path operators on
-device buffers (``DeviceBuffer`` and the ``op_*`` functions) and the
+device buffers (``DeviceBuffer`` and the ``op_*`` functions), those that serve
+several sequences (``CKvPages``, ``op_kv_append`` to ``op_sample``) and the
 synthetic model builder (``synth_model``).  The library must be built
 (``make -C unlimitedocr.c_amd``); there is no fallback implementation.
 """
