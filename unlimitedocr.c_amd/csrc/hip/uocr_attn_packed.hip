@@ -348,18 +348,18 @@ hipError_t launch(hipStream_t st, const uocr_packed_args &a) {
 /* Measured (us; wavefronts along queries x along keys, keys per tile; head_dim
  * 128; x: tiles of 128 rows, all heads, and one more for each sequence):
  *   heads x sequences x rows     x     4 x 1, 64   2 x 4, 32   4 x 2, 64
- *   10 x 1 x 64                  10         7.7         9.6         9.7
- *   10 x 1 x 932                 80        25.1        18.9        24.5
- *   10 x 1 x 2500               200        65.7        42.7        57.8
- *   32 x 1 x 700                192        20.4        21.0        20.8
- *   10 x 3 x 932                240        29.5        34.1        27.9
- *   10 x 12 x 200               300        15.6        21.6        22.1
- *   10 x 2 x 2000               330        57.0        59.6        50.3
- *   32 x 1 x 2000               512        57.2        78.8        57.1
- *   32 x 4 x 4001              4128       620.7       956.8       781.8   (845 TFLOP/s)
+ *   10 x 1 x 64                  10         7.4         9.4         8.7
+ *   10 x 1 x 932                 80        23.1        18.2        21.2
+ *   32 x 1 x 700                192        18.9        20.9        17.5
+ *   10 x 1 x 2500               200        51.3        38.6        42.3
+ *   10 x 3 x 932                240        24.1        30.9        22.6
+ *   10 x 12 x 200               300        15.6        22.4        22.1
+ *   10 x 2 x 2000               330        46.9        53.0        39.8
+ *   32 x 1 x 2000               512        53.1        71.9        49.9
+ *   32 x 4 x 4001              4128       599.6       865.4       649.4   (894 TFLOP/s)
  * Few tiles leave CUs or their second block idle: then wavefronts share the
  * walk over long keys; many want the tile with the fewest passes over K and V.
- * head_dim 64 goes alike (512 tiles: 37.1, 51.0, 34.1). */
+ * head_dim 64 goes alike (512 tiles: 35.2, 47.8, 33.0). */
 template <int D>
 hipError_t choose(hipStream_t st, const uocr_packed_args &a) {
     const uint64_t x = ((uint64_t)a.q_tokens / 128u + a.n_seqs) * a.heads, keys = a.k_tokens / a.n_seqs;
