@@ -466,6 +466,20 @@ def test_packed_attention_values_that_are_not_finite(gpu, dim, heads, n):
     packed_case(gpu, rng, heads, 1, dim, [n, 50], change=change)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,n", [(2, 400), (90, 400)])
+def test_packed_attention_not_finite_values_of_little_weight(gpu, dim, heads, n):
+    """A value that is not finite reaches every row that sees it, also where its weight rounds to zero in fp16."""
+    rng = np.random.default_rng(19)
+
+    def change(q, k, v):
+        q[:, :, 0], k[:, :, 0] = 2, 2
+        k[[10, 70, 130], 0, 0] = -6  # e^-24 of the others and less
+        v[10, 0, 5], v[70, 0, 6], v[130, 0, 7], v[70, 0, 8], v[130, 0, 8] = np.inf, -np.inf, np.nan, np.inf, -np.inf
+
+    packed_case(gpu, rng, heads, 1, dim, [n, 50], scale=1.5, change=change)
+
+
 def test_packed_attention_in_place(gpu):
     """out may be q, a value that is not finite among the rows that others do not see too."""
     rng = np.random.default_rng(18)

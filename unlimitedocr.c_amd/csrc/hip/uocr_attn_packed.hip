@@ -22,9 +22,9 @@ struct PackedGrid {
     float c; /* scale * log2(e) */
 };
 
-/* Not-finite values of V: 0 times them is NaN, so where a tile holds keys that
- * some rows do not see, they are taken out of the product and counted by a
- * second one, of 0 / 1 visibilities and these codes.  At most 64 keys a tile:
+/* Not-finite values of V: 0 times them is NaN, whether a row does not see them
+ * or their weight rounds to 0.  They are taken out of the product and counted by
+ * a second one, of 0 / 1 visibilities and these codes.  At most 64 keys a tile:
  * the counts of the three kinds do not run into each other, and all fit fp32
  * and fp16 exactly. */
 constexpr float CODE_PLUS = 1.0f, CODE_MINUS = 128.0f, CODE_NAN = 16384.0f;
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(64 * WQ * WG, 2) void k_packed_attention(PackedGrid
                 const uint2 hi = lds_read_tr4(vt + (key + 8u) * RB + 16u * swz_v(key + 8u, pc) + 8u * (lane & 1u));
                 return make_uint4(lo.x, lo.y, hi.x, hi.y);
             };
-            if (special && masked) {
+            if (special) {
                 for (u32 d = 0; d < D / 32; ++d) {
                     f32x16 n;
 #pragma unroll
