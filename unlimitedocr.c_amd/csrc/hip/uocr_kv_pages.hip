@@ -15,7 +15,7 @@ namespace {
 typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 
 /* Cached rows are read once: non-temporal loads, 154 against 285 us at 876 MB
- * of fp16 cache (5.7 TB/s) and 18.6 against 24.6 at 41 MB that the caches hold
+ * of fp16 cache and 18.6 against 24.6 at 41 MB that the caches hold
  * from call to call; Q8_0 pages, which need half the lines, 70 against 71. */
 __device__ __forceinline__ uint4 load_once(const uint8_t *p) {
     const u32x4 v = __builtin_nontemporal_load((const u32x4 *)p);
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
     constexpr u32 WLDS = 16 * ORS * 4 > 64 * D ? 16 * ORS * 4 : 64 * D; /* V tile, later the state */
     __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * WLDS];
     __shared__ float sml[4][2][16];
-    __shared__ __attribute__((aligned(16))) u32 scales[4][2][32];
+    __shared__ __attribute__((aligned(16))) float scales[4][2][32 * (D / 64)]; /* Q8_0: of the tokens' groups, those of V in units */
     __shared__ u32 arrived;
     const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 15u, gr = lane >> 4;
     const uocr_kv &kv = g.a.kv;
@@ -458,24 +458,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
             const u32 tok0 = x * PA_TILE + 32u * wave;
             valid = (u32)__ballot(p >= 0);
             const uint8_t *k = (const uint8_t *)kv.k, *v = (const uint8_t *)kv.v;
-            const u32 mask = (1u << kv.shift) - 1u, hrow = kvh << kv.shift;
-            auto row = [&](const uint8_t *pages, u32 i) {
-                const int pi = __shfl(p, (int)i);
-                const uint8_t *r = pages + ((uint64_t)(u32)pi * kv.page_stride + (uint64_t)(hrow + ((tok0 + i) & mask)) * D) * (Q8 ? 1u : 2u);
-                return pi >= 0 ? r : (const uint8_t *)g_zero_row;
-            };
+            /* Where the row of token lane % 32 stands in k and v.  V rows' places go from lane to lane, K rows' are formed anew
+             * from their pages: 146 us at 876 MB of fp16 cache, 154 with all formed anew; 53.3 at 272 MB of Q8_0, so 54.7, and
+             * 56.4 with all from lane to lane.  An absent token's scores count nothing, so a row of page 0 does for its key,
+             * but its value is read from a row of zeros. */
+            const u32 mask = (1u << kv.shift) - 1u, hrow = kvh << kv.shift, in_head = hrow + ((tok0 + (lane & 31u)) & mask);
+            const uint64_t values = p >= 0 ? (uint64_t)(u32)p * kv.page_stride + (uint64_t)in_head * D : 0u, bytes = values * (Q8 ? 1u : 2u);
 #pragma unroll
             for (u32 n = 0; n < 2; ++n) {
-                const uint8_t *r = row(k, 16u * n + col) + 16u * gr;
+                const int pk = max(__shfl(p, (int)(16u * n + col)), 0);
+                const uint8_t *r = k + ((uint64_t)(u32)pk * kv.page_stride + (uint64_t)(hrow + ((tok0 + 16u * n + col) & mask)) * D) * (Q8 ? 1u : 2u) + 16u * gr;
 #pragma unroll
                 for (u32 x2 = 0; x2 < NK; ++x2) kr[n * NK + x2] = load_once(r + 64u * x2);
             }
 #pragma unroll
-            for (u32 y = 0; y < NV; ++y) vr[y] = load_once(row(v, (64u / VL) * y + lane / VL) + 16u * (lane % VL));
+            for (u32 y = 0; y < NV; ++y) {
+                const u32 i = (64u / VL) * y + lane / VL;
+                const uint8_t *r = v + (((uint64_t)(u32)__shfl((int)(bytes >> 32), (int)i) << 32) | (u32)__shfl((int)bytes, (int)i));
+                vr[y] = load_once(((valid >> i) & 1u ? r : (const uint8_t *)g_zero_row) + 16u * (lane % VL));
+            }
             if constexpr (Q8) {
                 ksc = vsc = 0u;
                 if (p >= 0) {
-                    const uint64_t sat = (uint64_t)(u32)p * (kv.page_stride / 64u) + (uint64_t)(hrow + ((tok0 + (lane & 31u)) & mask)) * (D / 64u);
+                    const uint64_t sat = values / 64u;
                     if (D == 128) {
                         ksc = *(const u32 *)(kv.ks + sat);
                         vsc = *(const u32 *)(kv.vs + sat);
@@ -491,14 +496,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
         for (u32 x = ta; x < tb; ++x) {
             const u32 now = valid;
             float sc[8];
-            u32 sv[8]; /* Q8_0: the scales of V, where the scores are */
+            float sv[8][D / 64]; /* Q8_0: the scales of V, where the scores are */
             if (now != 0u) {
                 /* V to LDS, rows swizzled by pairs of 16-byte pieces so that the transposing reads touch all banks */
                 __builtin_amdgcn_wave_barrier();
-                if (Q8 && lane < 32u) {
-                    scales[wave][0][lane] = ksc;
-                    scales[wave][1][lane] = vsc;
-                }
                 if constexpr (Q8) {
                     const float top = fmaxf(fabsf(scale_of(vsc, 0)), fabsf(scale_of(vsc, 1)));
                     if (__any(top * unit > 1.0f)) {
@@ -511,6 +512,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                         for (u32 n = 0; n < D / 16; ++n)
 #pragma unroll
                             for (u32 i = 0; i < 4; ++i) o[n][i] *= by;
+                    }
+                    if (lane < 32u) {
+#pragma unroll
+                        for (u32 j = 0; j < D / 64; ++j) {
+                            scales[wave][0][lane * (D / 64) + j] = scale_of(ksc, j);
+                            scales[wave][1][lane * (D / 64) + j] = scale_of(vsc, j) * unit;
+                        }
                     }
                 }
                 auto swz = [](u32 key, u32 pc) { return key * (2u * D) + 16u * (pc ^ (D == 128 ? (key & 7u) << 1 : ((key >> 1) & 3u) << 1)); };
@@ -538,14 +546,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                             part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].x, kr[n * NK + j].y, 0x3c00u), qr[2 * j].v, part[j], 0, 0, 0);
                             part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dequant_q8(kr[n * NK + j].z, kr[n * NK + j].w, 0x3c00u), qr[2 * j + 1].v, part[j], 0, 0, 0);
                         }
-                        const uint4 k4 = *(const uint4 *)&scales[wave][0][16u * n + 4u * gr], v4 = *(const uint4 *)&scales[wave][1][16u * n + 4u * gr];
-                        const u32 ks[4] = {k4.x, k4.y, k4.z, k4.w}, vs[4] = {v4.x, v4.y, v4.z, v4.w};
+                        const float *ks = &scales[wave][0][(16u * n + 4u * gr) * (D / 64)], *vs = &scales[wave][1][(16u * n + 4u * gr) * (D / 64)];
 #pragma unroll
                         for (u32 i = 0; i < 4; ++i) {
-                            float v = part[0][i] * scale_of(ks[i], 0);
-                            if (D == 128) v = fmaf(part[D / 64 - 1][i], scale_of(ks[i], 1), v);
+                            float v = part[0][i] * ks[i * (D / 64)];
+                            if (D == 128) v = fmaf(part[D / 64 - 1][i], ks[i * (D / 64) + D / 64 - 1], v);
                             sc[4 * n + i] = v;
-                            sv[4 * n + i] = vs[i];
+#pragma unroll
+                            for (u32 j = 0; j < D / 64; ++j) sv[4 * n + i][j] = vs[i * (D / 64) + j];
                         }
                     } else {
                         f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -592,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(PagedGrid g) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -mc));
                 l += e;
 #pragma unroll
-                for (u32 j = 0; j < NP; ++j) p[j].h[i] = Q8 ? (h16)(e * (scale_of(sv[i], j) * unit)) : (h16)e;
+                for (u32 j = 0; j < NP; ++j) p[j].h[i] = Q8 ? (h16)(e * sv[i][j]) : (h16)e;
             }
 #pragma unroll
             for (u32 n = 0; n < D / 16; ++n) {
