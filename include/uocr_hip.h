@@ -322,8 +322,9 @@ UOCR_API int uocr_op_moe_ffn_rows_static(const uocr_op_moe_weights *m, const voi
  * page to the next are page_stride values (0: pages without gaps) and
  * page_stride / 64 scales, so that the layers of a model can share a page.
  * Limits: head_dim 64 or 128; page_tokens a power of two up to 65536;
- * page_stride a multiple of head_dim, at least the page; k and v on 16-byte,
- * scales on 4-byte boundaries; table_stride * page_tokens below 2^31. */
+ * page_stride a multiple of head_dim, at least the page, and n_pages of them up
+ * to 2^46 values; k and v on 16-byte, scales on 4-byte boundaries; table_stride
+ * * page_tokens below 2^31. */
 typedef struct uocr_op_kv_pages {
     uint32_t qtype;
     uint32_t kv_heads, head_dim;
@@ -339,8 +340,8 @@ typedef struct uocr_op_kv_pages {
 /* Writes the keys and values of `tokens` new tokens into their pages and
  * rotates queries and keys to their positions (split-half RoPE over the whole
  * head, angle = position * rope_theta^(-2 i / head_dim), formed in fp64 and
- * off by 2^-23 turns at most; rope_theta from 1, or 0: no rotation).  Token i belongs to
- * sequence seqs[i] (NULL: sequence i) at positions[i].  Rows are
+ * off by 2^-23 turns at most; rope_theta from 1, or 0: no rotation).  Token i
+ * belongs to sequence seqs[i] (NULL: sequence i) at positions[i].  Rows are
  * [heads][head_dim] fp16 (k, v: [kv_heads][head_dim]), q_stride .. v_stride
  * values from one token to the next (at least a row).  q NULL: no queries;
  * q_out may be q and k_out may be k (with the same stride); k_out NULL: the

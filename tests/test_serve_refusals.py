@@ -33,7 +33,7 @@ BAD_CACHES = [
     (dict(table_stride=0), "table_stride"), (dict(reserved0=1), "reserved0"), (dict(page_tokens=0), "power of two"),
     (dict(page_tokens=24), "power of two"), (dict(page_tokens=1 << 17), "power of two"),
     (dict(page_tokens=1 << 16, table_stride=1 << 15), "below 2^31"), (dict(page_stride=2 * 16 * 64 - 64), "page_stride"),
-    (dict(page_stride=2 * 16 * 64 + 32), "page_stride"), (dict(page_stride=1 << 41), "page_stride"), (dict(k=AT + 8), "16-byte"),
+    (dict(page_stride=2 * 16 * 64 + 32), "page_stride"), (dict(page_stride=1 << 45), "page_stride"), (dict(n_pages=(1 << 31) - 1, page_stride=1 << 16), "page_stride"), (dict(k=AT + 8), "16-byte"),
     (dict(v=AT + 2), "16-byte"), (dict(page_table=AT + 2), "16-byte"), (dict(qtype=3), "Q8_0 pages"),
     (dict(qtype=3, k_scales=AT), "Q8_0 pages"), (dict(qtype=3, k_scales=AT, v_scales=AT + 2), "Q8_0 pages"),
 ]

@@ -660,8 +660,8 @@ int pages_of(const uocr_op_kv_pages *c, const char *what, uocr_kv *kv) {
     }
     const uint64_t dense = (uint64_t)c->kv_heads * page * c->head_dim;
     const uint64_t stride = c->page_stride != 0u ? c->page_stride : dense;
-    if (stride < dense || stride % c->head_dim != 0u || stride > (1ull << 40)) {
-        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: page_stride is a multiple of head_dim of at least a page", what);
+    if (stride < dense || stride % c->head_dim != 0u || stride > (1ull << 46) / c->n_pages) {
+        return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: page_stride is a multiple of head_dim of at least a page, n_pages of them up to 2^46 values", what);
     }
     if (off(c->k, 16) || off(c->v, 16) || off(c->page_table, 4)) {
         return op_fail(UOCR_ERROR_INVALID_ARGUMENT, "%s: k and v stand on 16-byte boundaries, the table on 4", what);
