@@ -624,6 +624,22 @@ def test_sample_long_crowded_rows(gpu, f32):
         sample_case(gpu, x, f32, u=u, **s)
 
 
+@pytest.mark.parametrize("f32", [False, True], ids=["f16", "f32"])
+@pytest.mark.parametrize("vocab", [3000, 40003])
+def test_sample_flat_rows(gpu, f32, vocab):
+    """Logits within little of each other, some rows with most tokens masked or with a few far below, NaN between."""
+    rng = np.random.default_rng(26)
+    x = (rng.standard_normal((9, vocab)) * rng.choice([0.01, 0.1, 0.5], (9, 1))).astype(np.float32)
+    x[3, rng.random(vocab) < 0.97] = -np.inf
+    x[4, rng.random(vocab) < 0.5] = np.nan
+    x[5, ::3] -= 40
+    x[6, 512:] -= 3  # the first step is not like the others
+    x[7, :-512] -= 0.5
+    u = rng.uniform(0, 1, 9)
+    for s in (dict(p=0.9), dict(p=0.999999), dict(k=2000, p=0.5), dict(k=700), dict(k=vocab - 1), dict(p=0.5, t=3.0), dict(p=0.7, m=0.9), dict(p=0.9, t=0.05)):
+        sample_case(gpu, x, f32, u=u, **s)
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 16384), (1, 16385), (64, 32768), (64, 32769), (63, 20000), (128, 32768), (128, 32769), (2, 300007), (1, 1500000)])
 def test_sample_one_block_or_several(gpu, rows, vocab):
     """Sizes on both sides of where rows are shared, rows of more than 512 steps, each row with settings of its own."""

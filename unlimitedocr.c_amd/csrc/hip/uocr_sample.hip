@@ -20,7 +20,7 @@ constexpr u32 TAB = 64;                   /* 2^(i / TAB): 64 doubles, two to a p
 constexpr u32 MAX_CHUNKS = 64;
 constexpr u32 TOPS = 512;                 /* groups of steps whose largest logits bound top-k */
 constexpr u32 FEW = 128;                  /* values that are all counted against each other */
-constexpr u32 COUNTED = 512;              /* bins whose values are counted for top-p alone: weights from e^-8 on */
+constexpr float COUNTED = 8.0f;           /* values of top-p alone are counted to this distance, in temperatures */
 constexpr u64 DONE = ~0ull;               /* instead of a rank: the row has its token */
 
 /* Weights are integers in units of 2^-shift, shift = 62 - log2(vocab) rounded
@@ -34,6 +34,8 @@ struct Row {
     float top;     /* the largest logit */
     float scale;   /* bins per logit */
     float cut;     /* logits below are lighter than min_p */
+    float near;    /* distance to which values are counted */
+    float most;    /* the last bin that a logit above -inf can be in */
     u32 shift, k;
     float p;
     bool inf, use_k, use_p;
@@ -94,9 +96,12 @@ __device__ __forceinline__ void fill_table(double *tab, u32 shift) {
 }
 
 /* Bins of equal width below the largest logit, over the range where a weight
- * has a unit; the last one holds what has none. */
+ * has a unit, or down to the least of the row's first logits if that is less
+ * than half as far: flat rows would crowd few bins, and a crowded one takes 220
+ * us instead of 30.  The bin before the last then holds all from there down.
+ * The last one holds what has no unit. */
 __device__ __forceinline__ u32 bin_of(const Row &r, float x) {
-    return x == r.top ? 0u : (u32)fminf((r.top - x) * r.scale, (float)(BINS - 1u)); /* NaN: the last */
+    return x == r.top ? 0u : (u32)fminf((r.top - x) * r.scale, x > -INFINITY ? r.most : (float)(BINS - 1u)); /* NaN: the last */
 }
 
 /* The settings of row b; cut: the distance from the largest logit. */
@@ -112,6 +117,8 @@ __device__ __forceinline__ Row settings_of(const uocr_sample_args &a, u32 b, u32
     const float m = a.min_p != nullptr && a.min_p[b] > 0.0f ? fminf(a.min_p[b], 1.0f) : 0.0f;
     r.min_w = ldexp((double)m, (int)shift);
     r.cut = temp * logf(m); /* -inf without min_p */
+    r.near = COUNTED * temp;
+    r.most = (float)(BINS - 1u);
     r.k = a.top_k != nullptr && a.top_k[b] > 0 ? (u32)a.top_k[b] : 0u;
     r.p = a.top_p != nullptr ? a.top_p[b] : 1.0f;
     r.use_k = r.k != 0u && r.k < a.vocab;
@@ -119,12 +126,18 @@ __device__ __forceinline__ Row settings_of(const uocr_sample_args &a, u32 b, u32
     return r;
 }
 
-/* With the rank of the row's largest logit.  Where that is +inf, logits are
- * taken as 0 there and -inf elsewhere (value_of). */
-__device__ __forceinline__ void set_top(Row &r, u64 max_rank) {
+/* With the rank of the row's largest logit, and the least that is known (+inf:
+ * none).  Where the largest is +inf, logits are taken as 0 there and -inf elsewhere
+ * (value_of). */
+__device__ __forceinline__ void set_top(Row &r, u64 max_rank, float least) {
     r.top = of_key((u32)(max_rank >> IDX_BITS));
     r.inf = r.top == INFINITY;
     if (r.inf) r.top = 0.0f;
+    const float span = r.top - least;
+    if (!r.inf && span > 0.0f && span * r.scale < (float)(BINS / 2u)) {
+        r.scale = fminf(((float)BINS - 1.5f) / span, 1e30f);
+        r.most = (float)(BINS - 2u);
+    }
     /* below: lighter than min_p by more than the roundings here (2^-20 of the distance, and of the logit) */
     const float far = r.cut;
     r.cut = r.top + far - 1e-6f * (fabsf(r.top) + fabsf(far));
@@ -154,6 +167,13 @@ __device__ __forceinline__ void lane_load(const void *row, u32 id0, u32 vocab, f
 }
 __device__ __forceinline__ float largest_of(const float *x) {
     return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+}
+
+/* The least of the lane's logits that are not -inf, and `least`. */
+__device__ __forceinline__ float least_of(const float *x, float least) {
+#pragma unroll
+    for (u32 e = 0; e < E; ++e) least = fminf(least, x[e] > -INFINITY ? x[e] : INFINITY);
+    return least;
 }
 
 /* f(step, values) for the steps s0, s0 + stride, .. below s1, by a wavefront:
@@ -505,12 +525,16 @@ __device__ __forceinline__ void greedy(const uocr_sample_args &a, u32 b, u64 max
     if (a.probs != nullptr) a.probs[b] = max_rank == 0ull ? 0.0f : 1.0f;
 }
 
-/* The rank of the block's largest logit, from its lanes'. */
-__device__ __forceinline__ u64 largest(float best, u32 best_id, u64 *red) {
+/* The rank of the block's largest logit, and the least of its lanes'. */
+__device__ __forceinline__ u64 largest(float best, u32 best_id, float &least, u64 *red, u64 *red2) {
     u64 rank = wave_max64(best_id == 0xffffffffu ? 0ull : rank_of(best, best_id));
-    if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = rank;
+    least = -wave_max_dpp(-least);
+    if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = rank, red2[threadIdx.x >> 6] = __float_as_uint(least);
     __syncthreads();
-    for (u32 i = 0; i < blockDim.x / 64u; ++i) rank = red[i] > rank ? red[i] : rank;
+    for (u32 i = 0; i < blockDim.x / 64u; ++i) {
+        rank = red[i] > rank ? red[i] : rank;
+        least = fminf(least, __uint_as_float((u32)red2[i]));
+    }
     __syncthreads();
     return rank;
 }
@@ -566,7 +590,10 @@ __device__ __forceinline__ u64 lane_units(const Row &r, const double *tab, const
 }
 
 /* The lane's values into the histogram (the last bin's have no weight): counts
- * from `counted` bins, weights for top-p. */
+ * from `counted` bins, weights for top-p.  Without EXACT, NaN and -inf of a flat
+ * row go to the bin before the last, where their weights and places at the end
+ * change nothing. */
+template <bool EXACT>
 __device__ __forceinline__ void into_bins(const Row &r, const double *tab, const float *x, u32 counted, u32 *counts, u64 *weights) {
     float v[E];
 #pragma unroll
@@ -580,7 +607,7 @@ __device__ __forceinline__ void into_bins(const Row &r, const double *tab, const
         u32 bin[ILP];
         u64 w[ILP];
 #pragma unroll
-        for (u32 i = 0; i < ILP; ++i) bin[i] = bin_of(r, v[i]);
+        for (u32 i = 0; i < ILP; ++i) bin[i] = EXACT ? bin_of(r, v[i]) : v[i] == r.top ? 0u : (u32)fminf((r.top - v[i]) * r.scale, r.most);
         if (r.use_p) {
 #pragma unroll
             for (u32 i = 0; i < ILP; ++i) w[i] = units(weight(r, tab, v[i]));
@@ -632,20 +659,22 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
     const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6, vocab = a.vocab;
     const u32 steps = (vocab + STEP - 1u) / STEP, groups = min(steps, TOPS);
     float best = -INFINITY;
+    float least = INFINITY;
     u32 best_id = 0xffffffffu;
     sm.tops[t % TOPS] = 0u;
     __syncthreads();
     each_step<F32, ROW_U>(row, vocab, wave, steps, WAVES, [&](u32 s, const float *x) {
         const u32 top = key_of(step_largest(s, x, best, best_id));
+        if (s == wave) least = least_of(x, least); /* of the wavefront's first step */
         if (lane == 0u) sm.tops[s % TOPS] = max(sm.tops[s % TOPS], top); /* a group's steps are one wavefront's: TOPS is a multiple of WAVES */
     });
-    const u64 max_rank = largest(best, best_id, sm.red);
+    const u64 max_rank = largest(best, best_id, least, sm.red, sm.red2);
     Row r = settings_of(a, b, shift);
     if (max_rank == 0ull || !r.hot) {
         if (t == 0u) greedy(a, b, max_rank);
         return;
     }
-    set_top(r, max_rank);
+    set_top(r, max_rank, least);
     fill_table(sm.tab, r.shift);
     if (t == 0u) sm.n = 0u;
     __syncthreads();
@@ -677,7 +706,7 @@ __device__ void whole_row(const uocr_sample_args &a, u32 b, const void *row, u32
     if (!found && (r.use_k || r.use_p)) {
         for (u32 i = t; i < BINS; i += NT) sm.weight[i] = 0ull, sm.count[i] = 0u;
         __syncthreads();
-        each_step<F32, ROW_U>(row, vocab, wave, steps, WAVES, [&](u32, const float *x) { into_bins(r, sm.tab, x, BINS - 1u, sm.count, sm.weight); });
+        each_step<F32, ROW_U>(row, vocab, wave, steps, WAVES, [&](u32, const float *x) { into_bins<true>(r, sm.tab, x, BINS - 1u, sm.count, sm.weight); });
         __syncthreads();
         const u32 n0 = sm.count[2 * t], n1 = sm.count[2 * t + 1];
         const u64 w0 = sm.weight[2 * t], w1 = sm.weight[2 * t + 1];
@@ -771,6 +800,7 @@ struct Plan {
     u32 parts, run;                /* of this launch, [parts][rows] blocks: steps of each */
     Row *settings;                 /* [rows] */
     u64 *max_rank;                 /* [rows][chunks] */
+    float *least;                  /* [rows][chunks] */
     u32 *tops;                     /* [rows][steps]: keys of the steps' largest logits */
     u64 *weight;                   /* [rows][BINS] */
     u32 *count;                    /* [rows][BINS] */
@@ -897,7 +927,7 @@ __device__ __forceinline__ void chunk_values(const Plan &g, const void *row, con
 /* 1: the steps' and the chunk's largest logit; the row's histogram is cleared. */
 template <bool F32>
 __global__ __launch_bounds__(CT) void k_sample_max(Plan g) {
-    __shared__ u64 red[CWAVES];
+    __shared__ u64 red[CWAVES], red2[CWAVES];
     const u32 b = blockIdx.x, chunk = blockIdx.y, lane = threadIdx.x & 63u;
     if (g.cut)
         for (u32 i = chunk * CT + threadIdx.x; i < BINS; i += CT * g.parts) g.weight[(u64)b * BINS + i] = 0ull, g.count[(u64)b * BINS + i] = 0u;
@@ -908,24 +938,36 @@ __global__ __launch_bounds__(CT) void k_sample_max(Plan g) {
     }
     const void *row = row_at<F32>(g.a, b);
     float best = -INFINITY;
+    float least = INFINITY;
     u32 best_id = 0xffffffffu;
-    each_step<F32, 4>(row, g.a.vocab, chunk * g.run + (threadIdx.x >> 6), min(chunk * g.run + g.run, g.steps), CWAVES, [&](u32 s, const float *x) {
+    const u32 s0 = chunk * g.run + (u32)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    each_step<F32, 4>(row, g.a.vocab, s0, min(chunk * g.run + g.run, g.steps), CWAVES, [&](u32 s, const float *x) {
         const float top = step_largest(s, x, best, best_id);
+        if (s == s0) least = least_of(x, least); /* of the wavefront's first step */
         if (lane == 0u) g.tops[(u64)b * g.steps + s] = key_of(top);
     });
-    const u64 rank = largest(best, best_id, red);
-    if (threadIdx.x == 0u) g.max_rank[(u64)b * g.chunks + chunk] = rank;
+    const u64 rank = largest(best, best_id, least, red, red2);
+    if (threadIdx.x == 0u) g.max_rank[(u64)b * g.chunks + chunk] = rank, g.least[(u64)b * g.chunks + chunk] = least;
 }
 
 __device__ __forceinline__ u64 row_max(const Plan &g, u32 b) {
     return wave_max64((threadIdx.x & 63u) < g.chunks ? g.max_rank[(u64)b * g.chunks + (threadIdx.x & 63u)] : 0ull);
+}
+__device__ __forceinline__ float row_least(const Plan &g, u32 b) {
+    return -wave_max_dpp((threadIdx.x & 63u) < g.chunks ? -g.least[(u64)b * g.chunks + (threadIdx.x & 63u)] : -INFINITY);
+}
+
+/* Bins whose values are counted: all for top-k; for top-p alone only so many as a
+ * list might hold. */
+__device__ __forceinline__ u32 counted_bins(const Row &r) {
+    return r.use_k ? BINS - 1u : (u32)fminf(r.near * r.scale, (float)(BINS - 1u));
 }
 
 /* Below: in bins behind `last`, as a comparison tells (three bins' margin for
  * their roundings). */
 __device__ __forceinline__ float floor_of(const Row &r, u32 last) {
     const float floor = r.top - ((float)last + 3.0f) / r.scale;
-    return floor > -INFINITY && !r.inf ? floor : -INFINITY;
+    return floor > -INFINITY && !r.inf && !(last >= BINS - 2u && r.most < (float)(BINS - 1u)) ? floor : -INFINITY;
 }
 /* Above: in bins before `first`. */
 __device__ __forceinline__ float ceiling_of(const Row &r, u32 first) {
@@ -981,7 +1023,7 @@ __device__ __forceinline__ Found find_bins(const Plan &g, u32 b, const Row &r, u
     f.floor = floor_of(r, f.last);
     /* With both, top-p decides within top-k's values: all of them are looked at.  As many as a list holds are listed from
      * the first on: then nothing else needs to be looked at for the token. */
-    const bool known = r.use_k || f.last < COUNTED, all = (f.use_k && r.use_p) || (known && out[1] + out[3] <= LIST);
+    const bool known = f.last < counted_bins(r), all = (f.use_k && r.use_p) || (known && out[1] + out[3] <= LIST);
     f.first = all ? 0u : f.last;
     f.base_n = all ? 0ull : out[1];
     f.base_w = all ? 0ull : out[2];
@@ -992,7 +1034,7 @@ __device__ __forceinline__ Found find_bins(const Plan &g, u32 b, const Row &r, u
 /* 2: the histogram, in LDS and from there into the row's.  A bounded row only
  * needs its bound. */
 template <bool F32>
-__global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
+__global__ __launch_bounds__(CT, F32 ? 5 : 7) void k_sample_bins(Plan g) {
     __shared__ double tab[TAB];
     __shared__ u64 weights[BINS];
     __shared__ u32 counts[BINS];
@@ -1004,8 +1046,9 @@ __global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
     const bool listed = bounded(r, groups);
     if (listed && (chunk != 0u || t >= 64u)) return;
     const u64 max_rank = row_max(g, b);
+    const float least = listed ? INFINITY : row_least(g, b);
     if (max_rank == 0ull) return;
-    set_top(r, max_rank);
+    set_top(r, max_rank, least);
     if (listed) {
         u32 tops[TOPS / 64] = {};
         for (u32 s0 = 0; s0 < g.steps; s0 += TOPS) {
@@ -1024,8 +1067,8 @@ __global__ __launch_bounds__(CT) void k_sample_bins(Plan g) {
     }
     for (u32 i = t; i < BINS; i += CT) weights[i] = 0ull, counts[i] = 0u;
     __syncthreads();
-    const u32 counted = r.use_k ? BINS - 1u : COUNTED;
-    chunk_steps<F32>(g, row_at<F32>(g.a, b), mine, floor_of(r, BINS - 1u), [&](u32, u32, const float *x) { into_bins(r, tab, x, counted, counts, weights); }, [](u32) {});
+    const u32 counted = counted_bins(r);
+    chunk_steps<F32>(g, row_at<F32>(g.a, b), mine, floor_of(r, BINS - 1u), [&](u32, u32, const float *x) { into_bins<false>(r, tab, x, counted, counts, weights); }, [](u32) {});
     __syncthreads();
     for (u32 i = t; i < BINS; i += CT) {
         if (counts[i] != 0u) atomicAdd(&g.count[(u64)b * BINS + i], counts[i]);
@@ -1041,12 +1084,15 @@ __global__ __launch_bounds__(CT) void k_sample_list(Plan g) {
     const u32 b = blockIdx.x, chunk = blockIdx.y, t = threadIdx.x;
     const Steps mine = steps_of(g, b, chunk);
     Row r = g.settings[b];
+    if (!r.hot || (!r.use_k && !r.use_p)) return;
+    const bool listed = bounded(r, min(g.steps, TOPS));
     const u64 max_rank = row_max(g, b);
-    if (max_rank == 0ull || !r.hot || (!r.use_k && !r.use_p)) return;
-    set_top(r, max_rank);
+    const float least = listed ? INFINITY : row_least(g, b);
+    if (max_rank == 0ull) return;
+    set_top(r, max_rank, least);
     if (t == 0u) n = 0u;
     Found f;
-    if (bounded(r, min(g.steps, TOPS))) {
+    if (listed) {
         f = g.found[b];
         __syncthreads();
     } else {
@@ -1083,7 +1129,7 @@ __global__ __launch_bounds__(NT) void k_sample_cut(Plan g) {
     const u32 n = g.n[b];
     const u64 max_rank = row_max(g, b), listed = g.list[(u64)b * LIST + t];
     if (max_rank == 0ull || !r.hot) return;
-    set_top(r, max_rank);
+    set_top(r, max_rank, -INFINITY); /* no bins here */
     u64 thr = 0;
     if (f.any) {
         if (f.crowded || n > LIST) {
@@ -1122,7 +1168,7 @@ __global__ __launch_bounds__(CT) void k_sample_sums(Plan g) {
         return;
     }
     if (thr == DONE) return;
-    set_top(r, max_rank);
+    set_top(r, max_rank, -INFINITY); /* no bins here */
     const void *row = row_at<F32>(g.a, b);
     __syncthreads();
     const Keep keep = keep_from(r, thr);
@@ -1187,6 +1233,7 @@ size_t lay_out(Plan &g, u32 rows, u32 vocab, uint8_t *ws) {
     };
     g.settings = (Row *)take((size_t)rows * sizeof(Row));
     g.max_rank = (u64 *)take((size_t)rows * MAX_CHUNKS * 8u);
+    g.least = (float *)take((size_t)rows * MAX_CHUNKS * 4u);
     g.tops = (u32 *)take((size_t)rows * g.steps * 4u);
     g.weight = (u64 *)take((size_t)rows * BINS * 8u);
     g.count = (u32 *)take((size_t)rows * BINS * 4u);
