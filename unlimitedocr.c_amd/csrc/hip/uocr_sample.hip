@@ -1211,8 +1211,8 @@ bool by_one_block(u32 rows, u32 vocab) { return vocab <= (rows < MANY_ROWS ? ONE
 /* Blocks of a launch, all rows: where all values take little each, more of them
  * only have their own beginnings to pay for; where some rows' values take an
  * exponential and atomics each and others' nothing, the rows are cut finer.  192
- * mixed rows of 129,280 fp16 took 88.7 us so (before their lists were ordered by
- * buckets: 78.6), 91.1 and 91.7 with 1,536 and 3,000 for the heavy ones. */
+ * mixed rows of 129,280 fp16 took 88.7 us so, 91.1 and 91.7 with 1,536 and 3,000
+ * for the heavy ones (80.5 since the lists are ordered by buckets). */
 constexpr u32 LIGHT_BLOCKS = 768, HEAVY_BLOCKS = 2048;
 
 u32 parts_of(const Plan &g, u32 rows, u32 blocks) {
