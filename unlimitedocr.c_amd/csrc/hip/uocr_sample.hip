@@ -58,9 +58,9 @@ __device__ __forceinline__ u64 rank_of(float x, u32 id) {
 }
 
 /* A weight in units, not yet rounded: 2^shift exp((x - top) / temperature), as
- * 2^(n / TAB) from the table, a fifth-degree sum for the rest, f <= 1/2 (off
- * by 2^-54), and the exponent (never below -986).  fp64: next to a limit the last bits decide which
- * token it is. */
+ * 2^(n / TAB) from the table, a fifth-degree sum for the rest, f <= 1/2 (off by
+ * 2^-54), and the exponent (never below -986).  fp64: next to a limit the last
+ * bits decide which token it is. */
 __device__ __forceinline__ double weight(const Row &r, const double *tab, float x) {
     constexpr double L = 0.6931471805599453 / TAB;
     const double y = fmax(((double)x - (double)r.top) * r.c, -65536.0); /* NaN, too: no weight */
